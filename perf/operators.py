@@ -14,8 +14,8 @@ A pass is one of
 Cache layouts (R slots: the rows rounded up to 32; a tile is 32 slots).
   f32  K and V [slot][nkv hd]
   f16  K [slot][nkv hd]; V [tile][nkv hd][32], slot 16 a + 4 g + b of a tile at place 8 g + 4 a + b
-  mx8  blocks of 32 channels of a token's head: value = q 2^(x - 133), q a signed byte within +-127, x the smallest byte
-       for which the block's largest magnitude times 2^(133 - x) lies below 127.5; x = 255: a value was not finite.
+  mx8  blocks of 32 channels of a token's head: value = q 2^(x - 133), q within +-127 and held as the byte q + 128, x the
+       smallest byte for which the block's largest magnitude times 2^(133 - x) is below 127.5; 255: a value was not finite.
        K [nkv][tile][slot / 16][channel / 64][channel % 64 / 16][slot % 16][channel % 16], then x [nkv][slot][hd / 32]
        V [nkv][tile][i][g][n][e][a][b]: channel hd / 16 n + 2 i + e, slot 16 a + 4 g + b; x [nkv][tile][hd / 32][g][a][b]
 """
@@ -156,20 +156,20 @@ def slots_of(case, lo, hi):
 
 
 def quantise(x):
-    """x [..., hd] -> (bytes [..., hd] int8, scales [..., hd / 32] uint8); 64 bits, since values lie next to borders."""
+    """x [..., hd] -> (bytes [..., hd], scales [..., hd / 32]); 64 bits, since values lie next to borders."""
     b = x.double().unflatten(-1, (-1, 32))
     top = b.abs().amax(-1)
     e = torch.frexp(top)[1] + 126                        # top = m 2^(e - 126), 1/2 <= m < 1: top 2^(133 - e) in [64, 128)
     e = (e + (top * torch.exp2((133 - e).double()) >= 127.5)).clamp(0, 254).masked_fill(top == 0, 0)
     q = torch.round(b * torch.exp2((133 - e).double())[..., None])
     bad = ~torch.isfinite(top)
-    return q.masked_fill(bad[..., None], 0).to(torch.int8).flatten(-2), e.masked_fill(bad, 255).to(torch.uint8)
+    return (q.masked_fill(bad[..., None], 0) + 128).to(torch.uint8).flatten(-2), e.masked_fill(bad, 255).to(torch.uint8)
 
 
 def dequantise(q, e):
     """f32 values of the blocks (64 bits inside: 2^(x - 133) has no f32 of its own below 2^-126)."""
     s = torch.exp2(e.double() - 133.0).masked_fill(e == 255, math.nan)
-    return (q.unflatten(-1, (-1, 32)).double() * s[..., None]).flatten(-2).float()
+    return ((q.unflatten(-1, (-1, 32)).double() - 128.0) * s[..., None]).flatten(-2).float()
 
 
 def empty_cache(case, layers=1):
@@ -209,7 +209,7 @@ def put(case, cache, which, slots, x):
     flat, at = cache.view(-1), places(case, slots, which)
     if case.get("fmt", MX8) == MX8:
         q, e = quantise(x)
-        flat[at[0]] = q.view(torch.uint8)
+        flat[at[0]] = q
         flat[at[1]] = e
     else:
         flat[at] = x.to(cache.dtype)
@@ -219,7 +219,7 @@ def take(case, cache, which, slots):
     """Rows `slots` of one layer's cache as f32 [n][nkv][hd]."""
     flat, at = cache.view(-1), places(case, slots, which)
     if case.get("fmt", MX8) == MX8:
-        return dequantise(flat[at[0]].view(torch.int8), flat[at[1]])
+        return dequantise(flat[at[0]], flat[at[1]])
     return flat[at].float()
 
 
