@@ -50,7 +50,10 @@ constexpr float AX_LOG2E = 1.4426950408889634f;
 
 typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 
-template <int HD, bool F16, int RG>
+// TREE (atencion_arbol): the T rows are drafted tokens of a tree behind pos0 keys.  All of them see those keys (from their
+// window on), and of the drafted keys those that their mask names.  A value that is not finite reaches the rows that see its
+// key and no others (without TREE: every row of the block), and a row that sees no key is 0.
+template <int HD, bool F16, int RG, bool TREE = false>
 QP_DEV void attn_x_body(const QpAttnArgs& a) {
     constexpr int KS = HD / 32, DT = HD / 16;  // steps of 32 dimensions, tiles of 16 (DT dimensions per lane of 16)
     extern __shared__ float4 ax_lds[];
@@ -65,6 +68,7 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
     h8 qh[RG][KS], ql[RG][KS];
     float qs[RG];         // score = accumulator * qs (times the keys' scale), in units of log2
     int lim[RG], low[RG]; // keys low < key <= lim
+    uint64_t mrow[RG];    // TREE: the row's mask words
     bool alike = true;    // the operands so far are of like magnitudes (this lane's)
 #pragma unroll
     for (int r = 0; r < RG; r++) {
@@ -91,10 +95,16 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
         qs[r] = ax_pow2(e - 9) * a.scale * AX_LOG2E;
         lim[r] = (int)(pos0 + t);
         low[r] = a.swa && pos0 + t >= a.swa ? (int)(pos0 + t - a.swa) : -1;
+        if constexpr (TREE) {
+            const uint32_t p = a.where ? min(max(cptr<uint32_t>(a.where)[t], pos0), pos0 + T - 1) : pos0 + t;
+            low[r] = a.swa && p >= a.swa ? (int)(p - a.swa) : -1;
+            mrow[r] = a.mask + 4ull * t * a.mw;
+        }
     }
     // ---- the key tiles: keys kbeg .. kend in slots first .. (ring: then 0 ..), whole tiles of 32 slots
-    const uint32_t kend = a.cap ? pos0 + t_hi + 1 : min(pos0 + t_hi + 1, a.rows);
-    const uint32_t kbeg = a.swa && pos0 + t_lo + 1 > a.swa ? min(pos0 + t_lo + 1 - a.swa, kend) : 0;
+    const uint32_t last = TREE ? T - 1 : t_hi, early = TREE ? 0 : t_lo;
+    const uint32_t kend = a.cap ? pos0 + last + 1 : min(pos0 + last + 1, a.rows);
+    const uint32_t kbeg = a.swa && pos0 + early + 1 > a.swa ? min(pos0 + early + 1 - a.swa, kend) : 0;
     const uint32_t first = a.cap ? kbeg % a.cap : kbeg, nkey = a.cap ? min(kend - kbeg, a.cap) : kend - kbeg;
     const uint32_t end_a = a.cap ? min(first + nkey, a.cap) : first + nkey, end_b = first + nkey - end_a;
     const uint32_t ta = nkey ? (end_a + 31) / 32 - first / 32 : 0, nt = ta + (end_b + 31) / 32;
@@ -156,6 +166,27 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
         return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, m), __builtin_bit_cast(us2, w & 0x7fff7fffu)));
     };
 
+    // TREE: bits of the row's mask for the tile's 32 slots (drafted tokens only); whether the row sees the key in slot k
+    auto drafted = [&](const Tile& t, int r) __attribute__((always_inline)) -> uint32_t {
+        const int j = (int)t.slot + t.off - (int)pos0, w = j >> 5, sh = j & 31;
+        const uint32_t b0 = w >= 0 && w < (int)a.mw ? gload<uint32_t>(mrow[r] + 4ull * (uint32_t)w) : 0;
+        const uint32_t b1 = w + 1 >= 0 && w + 1 < (int)a.mw ? gload<uint32_t>(mrow[r] + 4ull * (uint32_t)(w + 1)) : 0;
+        return (uint32_t)((((uint64_t)b1 << 32) | b0) >> sh);
+    };
+    auto sees = [&](const Tile& t, int r, uint32_t k, uint32_t bits) __attribute__((always_inline)) {
+        const int key = (int)(t.slot + k) + t.off;
+        return t.slot + k >= t.lo && t.slot + k < t.hi && (key < (int)pos0 ? key > low[r] : ((bits >> k) & 1) != 0);
+    };
+    // all slots hold keys that every row of the block sees
+    auto all_see = [&](const Tile& t) __attribute__((always_inline)) {
+        if constexpr (TREE)
+            return t.slot >= t.lo && t.slot + 32 <= t.hi && (int)t.slot + 31 + t.off < (int)pos0 &&
+                   (!a.swa || (int)t.slot + t.off > (int)(pos0 + T - 1) - (int)a.swa);
+        else
+            return t.slot >= t.lo && t.slot + 32 <= t.hi && (int)t.slot + 31 + t.off <= (int)(pos0 + t_lo) &&
+                   (!a.swa || (int)t.slot + t.off > (int)(pos0 + t_hi) - (int)a.swa);
+    };
+
     f32x4 o[RG][DT];
     float m[RG], l[RG], p[RG][8], corr[RG];
     int ek = 0, ev = 0;     // the keys' and values' scale
@@ -168,12 +199,12 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
     }
     // softmax of the lane's 8 keys of each of its rows: scores s times unit (and qs), in units of log2
     auto softmax = [&](const Tile& t, const f32x4 (&s)[RG][2], auto Split, float unit) __attribute__((always_inline)) {
-        // all slots hold keys that every row of the block sees
-        const bool whole = t.slot >= t.lo && t.slot + 32 <= t.hi && (int)t.slot + 31 + t.off <= (int)(pos0 + t_lo) &&
-                           (!a.swa || (int)t.slot + t.off > (int)(pos0 + t_hi) - (int)a.swa);
+        const bool whole = all_see(t);
 #pragma unroll
         for (int r = 0; r < RG; r++) {
             const float c = Split.v ? qs[r] * unit : unit;
+            uint32_t bits = 0;
+            if constexpr (TREE) bits = whole ? 0 : drafted(t, r);
             float x[8], mx = -3.0e38f;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -181,7 +212,8 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
                 if (!whole) {
                     const uint32_t sl = t.slot + (j >> 2) * 16 + 4 * g + (j & 3);
                     const int key = (int)sl + t.off;
-                    x[j] = sl >= t.lo && sl < t.hi && key <= lim[r] && key > low[r] ? x[j] : -__builtin_inff();
+                    if constexpr (TREE) x[j] = sees(t, r, sl - t.slot, bits) ? x[j] : -__builtin_inff();
+                    else x[j] = sl >= t.lo && sl < t.hi && key <= lim[r] && key > low[r] ? x[j] : -__builtin_inff();
                 }
                 mx = fmaxf(mx, x[j]);
             }
@@ -209,6 +241,44 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
 #pragma unroll
             for (int d = 0; d < VL; d++) vw[d][j] &= keep;
         }
+    };
+    // TREE: the values of a tile with keys that not every row sees: those that are not finite make the channel NaN in the
+    // rows that see their key (the lane's own row and channels DT (4 g + x) + d), and are taken out of the product.
+    auto poison = [&](const Tile& t) __attribute__((always_inline)) {
+        if (all_see(t)) return;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int d = 0; d < DT; d++) bad |= !(fabsf(val(j, d)) < __builtin_inff());
+        if (!__any(bad)) return;
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            const uint32_t bits = drafted(t, r);
+            for (uint32_t k = 0; k < 32; k++) {
+                if (!sees(t, r, k, bits)) continue;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const uint32_t s = t.slot + k, c = kvh * HD + DT * (4 * g + x) + d;
+                        const float v = F16 ? h2f(gload<uint16_t>(a.vc + 2 * vt_index(s, kvd, c)))
+                                            : gload<float>(a.vc + 4 * ((uint64_t)s * kvd + c));
+                        if (!(fabsf(v) < __builtin_inff())) o[r][d][x] = __builtin_nanf("");
+                    }
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < VL; w++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                if constexpr (F16) {
+                    if ((vw[w][x] & 0x7c00u) == 0x7c00u) vw[w][x] &= 0xffff0000u;
+                    if ((vw[w][x] & 0x7c000000u) == 0x7c000000u) vw[w][x] &= 0xffffu;
+                } else if ((vw[w][x] & 0x7f800000u) == 0x7f800000u) {
+                    vw[w][x] = 0;
+                }
+            }
     };
     auto rescale = [&](float f) __attribute__((always_inline)) {
         bool same = f == 1.0f;
@@ -288,6 +358,7 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
         softmax(t, s, SkInt<1>(), F16 ? 1.0f : ax_pow2(ek - 9));
         // ---- O^T += V^T P^T
         mask_v(t);
+        if constexpr (TREE) poison(t);
         float vx[8];
         if constexpr (F16) {
 #pragma unroll
@@ -381,6 +452,7 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
             load_k(i + 4);
             softmax(t, s, SkInt<0>(), a.scale * AX_LOG2E);
             mask_v(t);
+            if constexpr (TREE) poison(t);
             rescale(1.0f);
             pv_f32();
             load_v(i + 4);
@@ -423,12 +495,13 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
             const float lw = ml[2 * at + 1], f = lw != 0.0f ? __builtin_amdgcn_exp2f(ml[2 * at] - M) : 0.0f;
             const float4 v = *reinterpret_cast<const float4*>(ol + at * LD + 4 * c);
             L += lw * f;
-            if (f != 0.0f) s = make_float4(s.x + v.x * f, s.y + v.y * f, s.z + v.z * f, s.w + v.w * f);
+            if (TREE ? lw != 0.0f : f != 0.0f) s = make_float4(s.x + v.x * f, s.y + v.y * f, s.z + v.z * f, s.w + v.w * f);
         }
         const uint32_t t = row / G, h = kvh * G + row % G;
         const uint64_t at = (uint64_t)t * a.nh + h;
         if (a.nsplit == 1) {
-            gstore<float4>(a.o + 4 * (at * HD + 4 * c), make_float4(s.x / L, s.y / L, s.z / L, s.w / L));
+            const bool none = TREE && L == 0.0f;
+            gstore<float4>(a.o + 4 * (at * HD + 4 * c), none ? make_float4(0, 0, 0, 0) : make_float4(s.x / L, s.y / L, s.z / L, s.w / L));
         } else {
             gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + 4 * c), s);
             if (c == 0) gstore<float2>(a.part_ml + 8 * (at * a.nsplit + blockIdx.z), make_float2(M, L));
@@ -442,6 +515,12 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
     KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void qp_attn_x_h##HD##_##NAME##_r2(         \
         QpAttnArgs a) { attn_x_body<HD, F16, 2>(a); }
 ATTN_X(64, f32, false) ATTN_X(128, f32, false) ATTN_X(64, f16, true) ATTN_X(128, f16, true)
+#define ATTN_T(HD, NAME, F16)                                                                                         \
+    KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void qp_attn_t_h##HD##_##NAME##_r1(         \
+        QpAttnArgs a) { attn_x_body<HD, F16, 1, true>(a); }                                                           \
+    KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void qp_attn_t_h##HD##_##NAME##_r2(         \
+        QpAttnArgs a) { attn_x_body<HD, F16, 2, true>(a); }
+ATTN_T(64, f32, false) ATTN_T(128, f32, false) ATTN_T(64, f16, true) ATTN_T(128, f16, true)
 
 // The shares' partial states of each (query, head) row -> o, in their order: grid rows, hd threads (at most 64 shares).
 KERNEL __launch_bounds__(128) void qp_attn_x_comb(QpAttnArgs a) {

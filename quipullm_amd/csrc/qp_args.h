@@ -198,7 +198,36 @@ typedef struct {
     // tcov: tokens the dispatch covers (none past them is computed)
     uint32_t nsplit, tcov;
     uint64_t part_o, part_ml;
+    // atencion_arbol: mask [T][mw] words, bit j % 32 of word j / 32 of row t: token t sees drafted token j (slot pos0 + j);
+    // where: 0, or the tokens' positions [T] (pos0 .. pos0 + T - 1), from which windows count
+    uint64_t mask, where;
+    uint32_t mw, pad;
 } QpAttnArgs;
+
+// ---------------------------------------------------------------- 8-bit caches, drafted trees (qp_cache.hip)
+#define QP_KV_F32 0
+#define QP_KV_F16 1
+#define QP_KV_MX8 2
+// norm_rope_kv: qo = rotated (and normed, qnorm != 0) q; the cache's slots (pos0 + t) mod cap = (rotated and normed k, v).
+// freq: base^(-2j/nrot), [nrot / 2]; pos: 0 (pos0 + t), or the tokens' positions.  tcov: tokens the dispatch covers.
+typedef struct {
+    uint64_t q, k, v, qo, kc, vc, qnorm, knorm, freq, pos, paso;
+    uint32_t hd, nh, nkv, neox, nrot, cap, fmt, rows, tcov;
+    float eps, esc;
+    uint32_t pad;
+} QpRopeKvArgs;
+// kv_read: rows of positions p0 .. p0 + n - 1 -> k, v [n][nkv hd], f32 (out 0) or f16 (out 1)
+typedef struct {
+    uint64_t kc, vc, k, v;
+    uint32_t hd, nkv, cap, fmt, rows, p0, n, out;
+} QpKvReadArgs;
+// kv_ramal: slot of pos0 + i <- slot of pos0 + idx[i], i < n, in each layer's K (cache[2 l]) and V (cache[2 l + 1])
+#define QP_RAMAL_LAYERS 64
+typedef struct {
+    uint64_t idx, paso;
+    uint32_t hd, nkv, cap, fmt, rows, n;
+    uint64_t cache[2 * QP_RAMAL_LAYERS];
+} QpRamalArgs;
 
 // Split-K decode attention with fused q/k norm + RoPE + KV append (one token).
 typedef struct {

@@ -81,11 +81,13 @@ enum Kid {
 #define M(name) K_##name,
 #define A(name) K_##name,
 #define T(name) K_##name,
+#define C(name) K_##name,
 #include "qp_kernel_list.inc"
 #undef K
 #undef M
 #undef A
 #undef T
+#undef C
     K_COUNT
 };
 const char* kNames[] = {
@@ -93,26 +95,30 @@ const char* kNames[] = {
 #define M(name) "qp_" #name,
 #define A(name) "qp_" #name,
 #define T(name) "qp_" #name,
+#define C(name) "qp_" #name,
 #include "qp_kernel_list.inc"
 #undef K
 #undef M
 #undef A
 #undef T
+#undef C
 };
 // The code objects (beside each other; one source file each) and which of them holds a kernel.
-constexpr int kObjects = 4;
+constexpr int kObjects = 5;
 const char* kObjectNames[kObjects] = {"quipu_kernels.hsaco", "quipu_small.hsaco", "quipu_attn.hsaco",
-                                        "quipu_tile.hsaco"};
+                                        "quipu_tile.hsaco", "quipu_cache.hsaco"};
 const uint8_t kObject[] = {
 #define K(name) 0,
 #define M(name) 1,
 #define A(name) 2,
 #define T(name) 3,
+#define C(name) 4,
 #include "qp_kernel_list.inc"
 #undef K
 #undef M
 #undef A
 #undef T
+#undef C
 };
 hipFunction_t g_fn[K_COUNT];
 
@@ -1010,6 +1016,246 @@ int op_atencion(const Ctx& c) {
                   a);
 }
 
+// ---- 8-bit caches and drafted trees (qp_cache.hip)
+// Bytes of the K (or V) cache of a layer.
+uint64_t kv_bytes(uint32_t fmt, bool v, uint32_t rows, uint32_t nkv, uint32_t hd) {
+    const uint64_t r32 = ((uint64_t)rows + 31) / 32 * 32, kvd = (uint64_t)nkv * hd;
+    if (fmt == QP_KV_MX8) return r32 * nkv * (hd + hd / 32);
+    return fmt == QP_KV_F16 ? (v ? r32 : rows) * kvd * 2 : rows * kvd * 4;
+}
+
+// The words that the ops over a cache share: head size and count, type, rows, ring.
+int kv_check(const char* op, uint32_t hd, uint32_t nkv, uint32_t cap, uint32_t fmt, uint32_t rows) {
+    if (hd != 64 && hd != 128) return fail(QP_E_ARG, "%s: head_dim %u (64 or 128 supported)", op, hd);
+    if (!nkv || nkv > 65535) return fail(QP_E_ARG, "%s: nkv=%u", op, nkv);
+    if (fmt > QP_KV_MX8) return fail(QP_E_ARG, "%s: cache type %u (0 f32, 1 f16, 2 mx8)", op, fmt);
+    if (!rows) return fail(QP_E_ARG, "%s: P.rows (cache slots) is 0", op);
+    if (cap > rows) return fail(QP_E_ARG, "%s: a ring of %u slots in a cache of %u", op, cap, rows);
+    return 0;
+}
+int kv_room(const char* op, uint64_t kc, uint64_t vc, uint32_t fmt, uint32_t rows, uint32_t nkv, uint32_t hd) {
+    if (!kc || !vc) return fail(QP_E_ARG, "%s: no cache bound", op);
+    if (int e = need_room(kc, kv_bytes(fmt, false, rows, nkv, hd), op, "the K cache")) return e;
+    return need_room(vc, kv_bytes(fmt, true, rows, nkv, hd), op, "the V cache");
+}
+
+// norm_rope_kv: P{hd, nh, nkv, neox, eps, nrot, esc, cap, fmt, rows}; [paso, q, k, v, qo, kc, vc, qnorm|0, knorm|0, freq|0,
+// pos|0]; (nh, T).  norm_rope of the T rows of q (into qo, which may be q) and of k, then kv_write of k's results and v.
+int op_norm_rope_kv(const Ctx& c) {
+    const char* op = "norm_rope_kv";
+    if (int e = need_bufs(c, 7, op)) return e;
+    QpRopeKvArgs a = {};
+    a.hd = c.U(0);
+    a.nh = c.U(1);
+    a.nkv = c.U(2);
+    a.neox = c.U(3);
+    a.eps = c.F(4);
+    a.nrot = c.U(5);
+    a.esc = c.U(6) ? c.F(6) : 1.0f;
+    a.cap = c.U(7);
+    a.fmt = c.U(8);
+    a.rows = c.U(9);
+    a.tcov = c.gy ? c.gy : 1;
+    if (int e = kv_check(op, a.hd, a.nkv, a.cap, a.fmt, a.rows)) return e;
+    if (!a.nh || a.nh > 65535 || a.nrot > a.hd || a.nrot % 2) return fail(QP_E_ARG, "%s: nh=%u nrot=%u", op, a.nh, a.nrot);
+    if (a.cap && a.tcov > a.cap) return fail(QP_E_ARG, "%s: %u tokens into a ring of %u slots", op, a.tcov, a.cap);
+    a.paso = c.B(0);
+    a.q = c.B(1);
+    a.k = c.B(2);
+    a.v = c.B(3);
+    a.qo = c.B(4);
+    a.kc = c.B(5);
+    a.vc = c.B(6);
+    a.qnorm = c.B(7);
+    a.knorm = c.B(8);
+    a.freq = c.B(9);
+    a.pos = c.B(10);
+    if (!a.paso || !a.q || !a.k || !a.v || !a.qo) return fail(QP_E_ARG, "%s: null binding", op);
+    if (a.nrot && !a.freq) return fail(QP_E_ARG, "%s: nrot=%u without a frequency table", op, a.nrot);
+    const uint64_t T = a.tcov, qb = 4 * T * a.nh * a.hd, kb = 4 * T * a.nkv * a.hd;
+    const struct { uint64_t p, n; const char* what; } need[] = {
+        {a.q, qb, "q"}, {a.qo, qb, "the output of q"}, {a.k, kb, "k"}, {a.v, kb, "v"}, {a.qnorm, 4ull * a.hd, "q's norm"},
+        {a.knorm, 4ull * a.hd, "k's norm"}, {a.freq, 2ull * a.nrot, "the frequency table"}, {a.pos, 4 * T, "the positions"}};
+    for (const auto& n : need)
+        if (n.p)
+            if (int e = need_room(n.p, n.n, op, n.what)) return e;
+    if (int e = kv_room(op, a.kc, a.vc, a.fmt, a.rows, a.nkv, a.hd)) return e;
+    return launch(K_norm_rope_kv, a.tcov, cdiv(a.nh + 2 * a.nkv, 512 / a.hd), 1, 256, 0, a);
+}
+
+// kv_read: P{hd, nkv, cap, fmt, rows, p0, n, out}; [paso|0, kc, vc, k, v].  The rows of positions p0 .. p0 + n - 1 as f32
+// (out 0) or f16 (out 1) [n][nkv hd].
+int op_kv_read(const Ctx& c) {
+    const char* op = "kv_read";
+    if (int e = need_bufs(c, 5, op)) return e;
+    QpKvReadArgs a = {};
+    a.hd = c.U(0);
+    a.nkv = c.U(1);
+    a.cap = c.U(2);
+    a.fmt = c.U(3);
+    a.rows = c.U(4);
+    a.p0 = c.U(5);
+    a.n = c.U(6);
+    a.out = c.U(7);
+    if (int e = kv_check(op, a.hd, a.nkv, a.cap, a.fmt, a.rows)) return e;
+    if (a.out > 1) return fail(QP_E_ARG, "%s: output type %u (0 f32, 1 f16)", op, a.out);
+    if (a.cap ? a.n > a.cap || (uint64_t)a.p0 + a.n > (1ull << 32) : (uint64_t)a.p0 + a.n > a.rows)
+        return fail(QP_E_ARG, "%s: positions %u + %u in a cache of %u slots", op, a.p0, a.n, a.cap ? a.cap : a.rows);
+    a.kc = c.B(1);
+    a.vc = c.B(2);
+    a.k = c.B(3);
+    a.v = c.B(4);
+    if (!a.k || !a.v) return fail(QP_E_ARG, "%s: null binding", op);
+    const uint64_t bytes = (uint64_t)a.n * a.nkv * a.hd * (a.out ? 2 : 4);
+    if (int e = need_room(a.k, bytes, op, "the keys' rows")) return e;
+    if (int e = need_room(a.v, bytes, op, "the values' rows")) return e;
+    if (int e = kv_room(op, a.kc, a.vc, a.fmt, a.rows, a.nkv, a.hd)) return e;
+    if (!a.n) return 0;
+    return launch(K_kv_read, grid_cap((uint64_t)a.n * a.nkv * a.hd / 2), 1, 1, 256, 0, a);
+}
+
+// kv_ramal: P{hd, nkv, cap, fmt, rows, n}; [paso, idx, kc, vc of each layer ...] (up to 64 layers).  The rows of drafted
+// tokens idx[0 .. n) (increasing; T, pos0 of Paso: drafted token j is in the slot of position pos0 + j) move to the slots of
+// positions pos0 .. pos0 + n - 1, in every layer's caches.
+int op_kv_ramal(const Ctx& c) {
+    const char* op = "kv_ramal";
+    if (int e = need_bufs(c, 4, op)) return e;
+    QpRamalArgs a = {};
+    a.hd = c.U(0);
+    a.nkv = c.U(1);
+    a.cap = c.U(2);
+    a.fmt = c.U(3);
+    a.rows = c.U(4);
+    a.n = c.U(5);
+    if (int e = kv_check(op, a.hd, a.nkv, a.cap, a.fmt, a.rows)) return e;
+    if (c.nb % 2 || c.nb > 2 + 2 * QP_RAMAL_LAYERS)
+        return fail(QP_E_ARG, "%s: %u bindings (Paso, idx, then K and V of 1 to %u layers)", op, c.nb, QP_RAMAL_LAYERS);
+    if (a.n > (a.cap ? a.cap : a.rows)) return fail(QP_E_ARG, "%s: %u rows in a cache of %u slots", op, a.n, a.cap ? a.cap : a.rows);
+    a.paso = c.B(0);
+    a.idx = c.B(1);
+    if (!a.paso || !a.idx) return fail(QP_E_ARG, "%s: null binding", op);
+    if (int e = need_room(a.idx, 4ull * a.n, op, "the path")) return e;
+    const uint32_t caches = c.nb - 2;
+    for (uint32_t i = 0; i < caches; i += 2) {
+        if (int e = kv_room(op, c.B(2 + i), c.B(3 + i), a.fmt, a.rows, a.nkv, a.hd)) return e;
+        a.cache[i] = c.B(2 + i);
+        a.cache[i + 1] = c.B(3 + i);
+    }
+    if (!a.n) return 0;
+    const uint32_t kvd = a.nkv * a.hd;
+    const uint32_t pieces = a.fmt == QP_KV_F32 ? kvd / 4 : a.fmt == QP_KV_F16 ? kvd : kvd + kvd / 32;
+    return launch(K_kv_ramal, cdiv(pieces, 256), caches, 1, 256, 0, a);
+}
+
+// The checks that atencion_mx8 and atencion_arbol share, the shares of the keys, and the launches.  parts: 0, or a buffer of
+// the caller's for the partial states of ns shares (a captured graph's own); ns = 0: as many as fill the device, in the
+// library's workspace (one while capturing a graph).
+int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool tree, uint32_t ns, uint64_t parts) {
+    if (int e = kv_check(op, a.hd, a.nkv, a.cap, fmt, a.rows)) return e;
+    if (!a.nh || a.nh % a.nkv || a.nh / a.nkv > 32) return fail(QP_E_ARG, "%s: nh=%u nkv=%u", op, a.nh, a.nkv);
+    const uint32_t T = c.gy ? c.gy : 1, G = a.nh / a.nkv;
+    if (a.cap && (!a.swa || (uint64_t)a.swa + T - 1 > a.cap))
+        return fail(QP_E_ARG, "%s: a ring of %u slots does not hold a window of %u for %u tokens", op, a.cap, a.swa, T);
+    if (!a.paso || !a.q || !a.o) return fail(QP_E_ARG, "%s: null binding", op);
+    const uint64_t r32 = ((uint64_t)a.rows + 31) / 32 * 32;
+    const uint64_t reach = fmt == QP_KV_MX8 ? r32 * a.hd : r32 * a.nkv * a.hd * (fmt == QP_KV_F16 ? 2 : 4);
+    if (reach >= (1ull << 31)) return fail(QP_E_ARG, "%s: %u slots (offsets past 31 bits)", op, a.rows);
+    if (int e = kv_room(op, a.kc, a.vc, fmt, a.rows, a.nkv, a.hd)) return e;
+    const uint64_t qb = 4ull * T * a.nh * a.hd;
+    if (int e = need_room(a.q, qb, op, "q")) return e;
+    if (int e = need_room(a.o, qb, op, "the output")) return e;
+    const uint64_t nrow = (uint64_t)T * G;
+    const uint32_t RG = nrow > 16 ? 2 : 1;
+    if (cdiv(nrow, 16 * RG) > 65535) return fail(QP_E_ARG, "%s: %u tokens in one call", op, T);
+    const uint32_t yb = cdiv(nrow, 16 * RG);
+    const uint64_t per = (uint64_t)T * a.nh * (4 * a.hd + 8);  // bytes of one share's partial states
+    if (ns > 64) return fail(QP_E_ARG, "%s: %u shares of the keys (at most 64)", op, ns);
+    if (ns > 1) {
+        if (!parts) return fail(QP_E_ARG, "%s: %u shares of the keys without a buffer for them", op, ns);
+        if (int e = need_room(parts, ns * per, op, "the shares' buffer")) return e;
+        a.part_o = parts;
+    } else if (!ns) {
+        const uint32_t cus = g_cus > 0 ? (uint32_t)g_cus : 1u;
+        const uint64_t keys = a.swa && (uint64_t)a.swa + T < a.rows ? a.swa + T : a.rows;
+        ns = cdiv(cus, a.nkv * yb);
+        if (ns > cdiv(keys, 128)) ns = cdiv(keys, 128);
+        if (ns > 64) ns = 64;
+        if (g_capturing && !g_noalloc) ns = 1;
+        if (g_noalloc && ns * per > QP_SCRATCH_BYTES) ns = 1;
+        if (ns > 1) {
+            if (int e = workspace(ns * per, &a.part_o)) return e;
+            if (a.part_o == g_split_memo.xs) g_split_memo.valid = false;  // (a split input kept there is overwritten)
+        }
+    }
+    a.f16 = fmt;
+    a.tcov = T;
+    a.nsplit = ns;
+    a.part_ml = ns > 1 ? a.part_o + 4ull * T * a.nh * ns * a.hd : 0;
+    static const Kid k8[2][2][2] = {{{K_attn_mx8_h64_causal_r1, K_attn_mx8_h64_causal_r2}, {K_attn_mx8_h128_causal_r1, K_attn_mx8_h128_causal_r2}},
+                                    {{K_attn_mx8_h64_tree_r1, K_attn_mx8_h64_tree_r2}, {K_attn_mx8_h128_tree_r1, K_attn_mx8_h128_tree_r2}}};
+    static const Kid kt[2][2][2] = {{{K_attn_t_h64_f32_r1, K_attn_t_h64_f32_r2}, {K_attn_t_h128_f32_r1, K_attn_t_h128_f32_r2}},
+                                    {{K_attn_t_h64_f16_r1, K_attn_t_h64_f16_r2}, {K_attn_t_h128_f16_r1, K_attn_t_h128_f16_r2}}};
+    const Kid k = fmt == QP_KV_MX8 ? k8[tree][a.hd == 128][RG == 2] : kt[fmt][a.hd == 128][RG == 2];
+    const uint32_t lds = 4 * RG * 16 * (a.hd + 4) * 4 + 4 * RG * 16 * 8;
+    if (int e = launch(k, a.nkv, yb, ns, 256, lds, a)) return e;
+    return ns == 1 ? 0 : launch(K_attn_mx8_comb, T * a.nh, 1, 1, a.hd, 0, a);
+}
+
+// atencion_mx8: atencion over an 8-bit cache: P{hd, nh, nkv, swa, escala, cap, 0, 0, 2, rows, nsplit}; [paso, q, kc, vc, o,
+// parts|0]; (nh, T).
+int op_atencion_mx8(const Ctx& c) {
+    const char* op = "atencion_mx8";
+    if (int e = need_bufs(c, 5, op)) return e;
+    QpAttnArgs a = {};
+    a.hd = c.U(0);
+    a.nh = c.U(1);
+    a.nkv = c.U(2);
+    a.swa = c.U(3);
+    a.scale = c.F(4);
+    a.cap = c.U(5);
+    a.rows = c.U(9);
+    if (c.U(6) || c.U(7)) return fail(QP_E_ARG, "%s: bidirectional / non-causal modes are not supported", op);
+    if (c.U(8) != QP_KV_MX8) return fail(QP_E_ARG, "%s: cache type %u (2: mx8)", op, c.U(8));
+    a.paso = c.B(0);
+    a.q = c.B(1);
+    a.kc = c.B(2);
+    a.vc = c.B(3);
+    a.o = c.B(4);
+    return attn_cache(op, c, a, QP_KV_MX8, false, c.U(10), c.B(5));
+}
+
+// atencion_arbol: P{hd, nh, nkv, swa, escala, cap, fmt, rows, nsplit}; [paso, q, kc, vc, o, mask, pos|0, parts|0]; (nh, T).
+// The T tokens of Paso are drafted continuations of the pos0 keys before them, drafted token j in the slot of position
+// pos0 + j: token t sees those pos0 keys (swa: the ones above pos[t] - swa) and drafted token j where bit j % 32 of word
+// j / 32 of row t of mask [T][ceil(T / 32)] is set.
+int op_atencion_arbol(const Ctx& c) {
+    const char* op = "atencion_arbol";
+    if (int e = need_bufs(c, 6, op)) return e;
+    QpAttnArgs a = {};
+    a.hd = c.U(0);
+    a.nh = c.U(1);
+    a.nkv = c.U(2);
+    a.swa = c.U(3);
+    a.scale = c.F(4);
+    a.cap = c.U(5);
+    a.rows = c.U(7);
+    a.paso = c.B(0);
+    a.q = c.B(1);
+    a.kc = c.B(2);
+    a.vc = c.B(3);
+    a.o = c.B(4);
+    a.mask = c.B(5);
+    a.where = c.B(6);
+    const uint32_t T = c.gy ? c.gy : 1;
+    a.mw = cdiv(T, 32);
+    if (!a.mask) return fail(QP_E_ARG, "%s: no mask bound", op);
+    if (a.swa && !a.where) return fail(QP_E_ARG, "%s: a window without the tokens' positions", op);
+    if (int e = need_room(a.mask, 4ull * T * a.mw, op, "the mask")) return e;
+    if (a.where)
+        if (int e = need_room(a.where, 4ull * T, op, "the positions")) return e;
+    return attn_cache(op, c, a, c.U(6), true, c.U(8), c.B(7));
+}
+
 // swiglu (gpu.js:570-582): P{F}; [paso, g, u].
 int op_swiglu(const Ctx& c) {
     if (int e = need_bufs(c, 3, "swiglu")) return e;
@@ -1743,6 +1989,11 @@ void register_ops() {
     v.push_back({"norm_rope", op_norm_rope});
     v.push_back({"kv_write", op_kv_write});
     v.push_back({"atencion", op_atencion});
+    v.push_back({"norm_rope_kv", op_norm_rope_kv});
+    v.push_back({"kv_read", op_kv_read});
+    v.push_back({"kv_ramal", op_kv_ramal});
+    v.push_back({"atencion_mx8", op_atencion_mx8});
+    v.push_back({"atencion_arbol", op_atencion_arbol});
     v.push_back({"swiglu", op_swiglu});
     v.push_back({"geglu", op_geglu});
     v.push_back({"escalar", [](const Ctx& c) { return op_scale(c, false); }});
