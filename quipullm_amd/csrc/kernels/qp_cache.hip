@@ -258,57 +258,332 @@ QP_DEV f32x4 mx_mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f
 
 constexpr float MX_LOG2E = 1.4426950408889634f;
 
-// A workgroup takes 16 RG (query, head) rows of one KV head and a share of the key tiles, dealt to its four wavefronts, each
-// with a softmax state of its own; they meet in LDS.  Scores are S^T = K Q^T and outputs O^T += V^T P^T with
-// v_mfma_f32_16x16x32_f16; queries and probabilities are f16 high and low parts (22 bits) below a power of two, keys and
-// values q 2^(x - E + 5) with one E of the wavefront each (16 times its first tile's largest), exact and normal for
-// x - E = -19 .. 0.  A wavefront takes its remaining tiles with the f32 matrix instruction (an eighth of the rate) where that
-// does not hold: a block of a tile lies outside that range, or a query's element is not 0 and below 2^-20 of its row's
-// largest (its part would lose bits), or not finite.  So no row loses bits to a key that it does not see.
-template <int HD, int RG, bool TREE>
+// Scores are S^T = K Q^T and outputs O^T += V^T P^T with v_mfma_f32_16x16x32_f16: a lane holds 8 scores of one row, which are its
+// operand of the second product.  Queries and probabilities are f16 high and low parts (22 bits) below a power of two.  Keys and
+// values are q 2^(x - E + 5) with an E of their own, exact and normal for x - E = -19 .. 0; a tile with blocks outside that
+// range moves E (and the sums so far with it).  Where no E will do (blocks of one tile further apart than 2^19, or not finite;
+// eight inputs of a query that are all below 2^-16 of its largest, whose parts would lose bits, or not finite), the workgroup
+// computes its rows with the f32 matrix instruction instead (attn_mx8_f32, some ten times slower).  So no row loses bits to a
+// key that it does not see.
+//
+// The softmax's reference m of a row follows its largest score only when a tile passes it by 2^MX_LAG: until then
+// probabilities of up to 2^MX_LAG are summed as they are, and no wavefront exchanges maxima or rescales its outputs.
+constexpr float MX_LAG = 3.0f, MX_UP = 0x1p12f;  // probabilities times MX_UP: below 2^15
+
+// What a wavefront works on.  WIDE: a workgroup takes 64 RG (query, head) rows of one KV head, 16 RG for each of its four
+// wavefronts, and all of them take all tiles of its share of the keys; else all have the same 16 RG rows.
+template <int HD, int RG, bool TREE, bool WIDE>
+struct MxWork {
+    static constexpr int CC = HD / 64, KS = HD / 32, DT = HD / 16, NB = HD / 32;
+    struct Tile { uint32_t slot, lo, hi; int off; };  // 32 slots from slot on; lo .. hi of them hold keys slot + off
+    uint32_t lane, wave, g, n16, T, pos0, G, kvh, nrow, R;
+    uint32_t b0, b_lo, b_hi, r0, t_lo, t_hi;  // the workgroup's rows and their tokens, the wavefront's
+    uint32_t kbeg, first, end_a, end_b, ta, i0, i1;
+    uint64_t hk, hx;                          // the head's bytes and scales in a cache
+    int lim[RG], low[RG];                     // the lane's rows see keys low < key <= lim
+    uint64_t mrow[RG];                        // TREE: and the drafted ones of their mask words
+    const QpAttnArgs& a;
+
+    QP_DEV MxWork(const QpAttnArgs& args) : a(args) {
+        lane = threadIdx.x & 63, g = lane >> 4, n16 = lane & 15;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        T = min(paso_T(a.paso), a.tcov), pos0 = paso_pos(a.paso);
+        G = a.nh / a.nkv, kvh = blockIdx.x, nrow = T * G, R = mx_slots(a.rows);
+        // long prompts: the blocks with the most keys first, then those with the fewest on (two workgroups share a CU)
+        const uint32_t y = blockIdx.y, ny = gridDim.y, blk = TREE ? y : y < (ny + 1) / 2 ? ny - 1 - y : y - (ny + 1) / 2;
+        b0 = blk * (WIDE ? 64 * RG : 16 * RG);
+        r0 = b0 + (WIDE ? wave * 16 * RG : 0);
+        if (b0 >= nrow) return;
+        b_lo = b0 / G, b_hi = (min(b0 + (WIDE ? 64 * RG : 16 * RG), nrow) - 1) / G;
+        t_lo = min(r0, nrow - 1) / G, t_hi = (min(r0 + 16 * RG, nrow) - 1) / G;
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            const uint32_t t = row(r) / G;
+            uint32_t p = pos0 + t;
+            if constexpr (TREE) {
+                if (a.where) p = min(max(cptr<uint32_t>(a.where)[t], pos0), pos0 + T - 1);
+                mrow[r] = a.mask + 4ull * t * a.mw;
+            }
+            lim[r] = (int)p;
+            low[r] = a.swa && p >= a.swa ? (int)(p - a.swa) : -1;
+        }
+        // the key tiles: keys kbeg .. kend in slots first .. (ring: then 0 ..), whole tiles of 32 slots
+        const uint32_t last = TREE ? T - 1 : b_hi, early = TREE ? 0 : b_lo;
+        const uint32_t kend = a.cap ? pos0 + last + 1 : min(pos0 + last + 1, a.rows);
+        kbeg = a.swa && pos0 + early + 1 > a.swa ? min(pos0 + early + 1 - a.swa, kend) : 0;
+        first = a.cap ? kbeg % a.cap : kbeg;
+        const uint32_t nkey = a.cap ? min(kend - kbeg, a.cap) : kend - kbeg;
+        end_a = a.cap ? min(first + nkey, a.cap) : first + nkey, end_b = first + nkey - end_a;
+        ta = nkey ? (end_a + 31) / 32 - first / 32 : 0;
+        const uint32_t nt = ta + (end_b + 31) / 32, per = (nt + a.nsplit - 1) / a.nsplit;
+        i0 = blockIdx.z * per, i1 = min(nt, i0 + per);
+        hk = (uint64_t)kvh * R * HD, hx = (uint64_t)a.nkv * R * HD + (uint64_t)kvh * R * NB;
+    }
+    // the lane's row of group r (past the last: the last), and its query from the lane's inputs on
+    QP_DEV uint32_t row(int r) const { return min(r0 + r * 16 + n16, nrow - 1); }
+    QP_DEV uint64_t query(int r) const {
+        const uint32_t rc = row(r);
+        return a.q + 4 * (((uint64_t)(rc / G) * a.nh + kvh * G + rc % G) * HD + 16 * g);
+    }
+    QP_DEV Tile tile(uint32_t i) const {
+        if (i < ta) return {(first / 32 + i) * 32, first, end_a, (int)(kbeg - first)};
+        return {(i - ta) * 32, 0, end_b, (int)(kbeg + a.cap - first)};
+    }
+    // slot k of the tile holds a key; all do
+    QP_DEV bool held(const Tile& t, uint32_t k) const { return t.slot + k >= t.lo && t.slot + k < t.hi; }
+    QP_DEV bool full(const Tile& t) const { return t.slot >= t.lo && t.slot + 32 <= t.hi; }
+    // TREE: bits of the lane's row's mask for the tile's 32 slots (drafted tokens only)
+    QP_DEV uint32_t drafted(const Tile& t, int r) const {
+        if constexpr (!TREE) return 0;
+        const int j = (int)t.slot + t.off - (int)pos0, w = j >> 5, sh = j & 31;
+        const uint32_t w0 = w >= 0 && w < (int)a.mw ? gload<uint32_t>(mrow[r] + 4ull * (uint32_t)w) : 0;
+        const uint32_t w1 = w + 1 >= 0 && w + 1 < (int)a.mw ? gload<uint32_t>(mrow[r] + 4ull * (uint32_t)(w + 1)) : 0;
+        return (uint32_t)((((uint64_t)w1 << 32) | w0) >> sh);
+    }
+    // the lane's row sees the key in slot k of the tile
+    QP_DEV bool sees(const Tile& t, int r, uint32_t k, uint32_t bits) const {
+        const int key = (int)(t.slot + k) + t.off;
+        if constexpr (TREE) return held(t, k) & (key < (int)pos0 ? key > low[r] : ((bits >> k) & 1) != 0);
+        else return held(t, k) & (key <= lim[r]) & (key > low[r]);
+    }
+    // all slots hold keys that all rows of tokens lo .. hi see
+    QP_DEV bool all_see(const Tile& t, uint32_t lo, uint32_t hi) const {
+        const int k0 = (int)t.slot + t.off;
+        return full(t) && k0 + 31 <= (int)pos0 + (TREE ? -1 : (int)lo) && (!a.swa || k0 > (int)(pos0 + (TREE ? T - 1 : hi)) - (int)a.swa);
+    }
+    // some row of the wavefront may see a key of the tile
+    QP_DEV bool wanted(const Tile& t) const {
+        const int k0 = (int)t.slot + t.off;
+        return r0 < nrow && (TREE || (k0 <= (int)(pos0 + t_hi) && (!a.swa || k0 + 31 > (int)(pos0 + t_lo) - (int)a.swa)));
+    }
+    // Channels c .. c + 3 of (query, head) row `row` from its state (m, l): the output, or this share's partial state.
+    QP_DEV void put(uint32_t row, uint32_t c, float4 s, float m, float l) const {
+        const uint64_t at = (uint64_t)(row / G) * a.nh + kvh * G + row % G;
+        if (a.nsplit == 1) {
+            gstore<float4>(a.o + 4 * (at * HD + c), l == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(s.x / l, s.y / l, s.z / l, s.w / l));
+        } else {
+            gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + c), s);
+            if (c == 0) gstore<float2>(a.part_ml + 8 * (at * a.nsplit + blockIdx.z), make_float2(m, l));
+        }
+    }
+};
+
+// A wavefront's softmax state.  o: row n16 of group r, channels DT (4 g + x) + d in o[r][d][x].
+template <int HD, int RG>
+struct MxState {
+    static constexpr int DT = HD / 16;
+    f32x4 o[RG][DT];
+    float m[RG], l[RG], p[RG][8];
+    bool far;  // some row's m lies past 2^20
+
+    QP_DEV void start() {
+        far = false;
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            m[r] = -3.0e38f;
+            l[r] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[r][d] = f32x4{0, 0, 0, 0};
+        }
+    }
+    // The probabilities p of the lane's 8 keys of each row, from the accumulators s (scores: times c, in units of log2).
+    template <class W>
+    QP_DEV void softmax(const W& w, const typename W::Tile& t, f32x4 (&s)[RG][2], const float (&c)[RG]) {
+        if (!w.all_see(t, w.t_lo, w.t_hi)) {
+#pragma unroll
+            for (int r = 0; r < RG; r++) {
+                const uint32_t bits = w.drafted(t, r);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    s[r][j >> 2][j & 3] = w.sees(t, r, (j >> 2) * 16 + 4 * w.g + (j & 3), bits) ? s[r][j >> 2][j & 3] : -__builtin_inff();
+            }
+        }
+        float mx[RG];
+        bool past = false;
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            mx[r] = s[r][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) mx[r] = fmaxf(mx[r], s[r][j >> 2][j & 3]);
+            past = past | (mx[r] * c[r] > m[r] + MX_LAG);
+        }
+        if (__any(past)) {
+            bool b = false;
+#pragma unroll
+            for (int r = 0; r < RG; r++) {
+                mx[r] = fmaxf(mx[r], bfly_f<4>(mx[r], w.lane));
+                mx[r] = fmaxf(mx[r], bfly_f<5>(mx[r], w.lane));
+                const float mn = fmaxf(m[r], mx[r] * c[r]), f = __builtin_amdgcn_exp2f(m[r] - mn);
+                m[r] = mn;
+                l[r] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) o[r][d][x] *= f;
+                b = b | (fabsf(mn) > 0x1p20f && mn > -3.0e38f);
+            }
+            far = __any(b) != 0;
+        }
+        if (far) {  // (s c - m in one rounding could be as large as half of m's last place)
+#pragma unroll
+            for (int r = 0; r < RG; r++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+#pragma clang fp contract(off)
+                    const float x = s[r][j >> 2][j & 3] * c[r];
+                    p[r][j] = __builtin_amdgcn_exp2f(x - m[r]);
+                }
+        } else {
+#pragma unroll
+            for (int r = 0; r < RG; r++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) p[r][j] = __builtin_amdgcn_exp2f(fmaf(s[r][j >> 2][j & 3], c[r], -m[r]));
+        }
+#pragma unroll
+        for (int r = 0; r < RG; r++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) l[r] += p[r][j];
+    }
+    // A value that is not finite reaches the rows that see its key, and no others: the lane's channels (which are of one
+    // block) become NaN in the rows that see a key of the tile whose block is NaN.
+    template <class W>
+    QP_DEV void poison(const W& w, const typename W::Tile& t) {
+        const uint64_t xs = w.a.vc + w.hx + (uint64_t)t.slot * W::NB + (DT * 4 * w.g / 32) * 32;
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            const uint32_t bits = w.drafted(t, r);
+            bool nan = false;
+#pragma unroll 1
+            for (uint32_t i = 0; i < 32; i++) {  // byte i: lane group i / 8, value i % 8
+                const uint32_t k = ((i >> 2) & 1) * 16 + 4 * (i >> 3) + (i & 3);
+                nan |= w.sees(t, r, k, bits) && gload<uint8_t>(xs + i) == MX_NAN;
+            }
+            if (nan) {
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[r][d] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            }
+        }
+    }
+    QP_DEV void sum_l(uint32_t lane) {
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            l[r] += bfly_f<4>(l[r], lane);
+            l[r] += bfly_f<5>(l[r], lane);
+        }
+    }
+    QP_DEV float4 out4(int r, int x, int d, int back) const {  // channels DT (4 g + x) + d .. d + 3, times 2^back
+        return make_float4(__builtin_ldexpf(o[r][d][x], back), __builtin_ldexpf(o[r][d + 1][x], back),
+                           __builtin_ldexpf(o[r][d + 2][x], back), __builtin_ldexpf(o[r][d + 3][x], back));
+    }
+    template <class W>
+    QP_DEV void put_all(const W& w, int back) const {
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            const uint32_t row = w.r0 + r * 16 + w.n16;
+            if (row >= w.nrow) continue;
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+#pragma unroll
+                for (int d = 0; d < DT; d += 4) w.put(row, DT * (4 * w.g + x) + d, out4(r, x, d, back), m[r], l[r]);
+        }
+    }
+};
+
+// The workgroup's rows in f32, its share of the keys from the first tile on.  Not WIDE: by the first wavefront alone.
+template <int HD, int RG, bool TREE, bool WIDE>
+__device__ __attribute__((noinline)) void attn_mx8_f32(const __attribute__((address_space(4))) QpAttnArgs* args) {
+    const QpAttnArgs a = *args;
+    using W = MxWork<HD, RG, TREE, WIDE>;
+    const W w(a);
+    if (WIDE ? w.r0 >= w.nrow : w.wave != 0) return;
+    MxState<HD, RG> st;
+    st.start();
+    const float scale = a.scale * MX_LOG2E, sign = scale < 0.0f ? -1.0f : 1.0f;
+    float c[RG];
+#pragma unroll
+    for (int r = 0; r < RG; r++) c[r] = fmaxf(fabsf(scale), 1.2e-38f);
+    const uint64_t kb = a.kc + w.hk + w.lane * 16, vb = a.vc + w.hk + w.lane * 16, kx = a.kc + w.hx, vx = a.vc + w.hx;
+    for (uint32_t i = w.i0; i < w.i1; i++) {
+        const typename W::Tile t = w.tile(i);
+        if (!w.wanted(t)) continue;
+        f32x4 s[RG][2];
+#pragma unroll
+        for (int r = 0; r < RG; r++) s[r][0] = s[r][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll 1
+            for (int cc = 0; cc < W::CC; cc++) {
+                const u32x4 k = gload<u32x4>(kb + (uint64_t)t.slot * HD + (h * W::CC + cc) * 1024);
+                const uint32_t x = gload<uint8_t>(kx + ((uint64_t)t.slot + h * 16 + w.n16) * W::NB + 2 * cc + (w.g >> 1));
+#pragma unroll
+                for (int b = 0; b < 16; b++)
+#pragma unroll
+                    for (int r = 0; r < RG; r++)
+                        s[r][h] = mx_mfma(mx_value((k[b >> 2] >> (8 * (b & 3))) & 255, x), gload<float>(w.query(r) + cc * 256 + 4 * b) * sign, s[r][h]);
+            }
+        st.softmax(w, t, s, c);
+        const bool whole = w.all_see(t, w.t_lo, w.t_hi);
+        uint32_t x[8];
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] = gload<uint8_t>(vx + (uint64_t)t.slot * W::NB + (w.n16 * W::DT / 32) * 32 + w.g * 8 + j);
+            bad = bad | (x[j] == MX_NAN);
+            if (!whole && (x[j] == MX_NAN || !w.held(t, (j >> 2) * 16 + 4 * w.g + (j & 3)))) x[j] = 0;
+        }
+        if (!whole && __any(bad)) st.poison(w, t);
+#pragma unroll
+        for (int d = 0; d < W::DT; d++) {
+            const uint64_t at = vb + (uint64_t)t.slot * HD + (d >> 1) * 1024 + 8 * (d & 1);
+            const uint2 v = gload<uint2>(at);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int r = 0; r < RG; r++)
+                    st.o[r][d] = mx_mfma(mx_value(((j < 4 ? v.x : v.y) >> (8 * (j & 3))) & 255, x[j]), st.p[r][j], st.o[r][d]);
+        }
+    }
+    st.sum_l(w.lane);
+    st.put_all(w, 0);
+}
+
+template <int HD, int RG, bool TREE, bool WIDE>
 QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
-    constexpr int CC = HD / 64, KS = HD / 32, DT = HD / 16, NB = HD / 32;
+    using W = MxWork<HD, RG, TREE, WIDE>;
+    using Tile = typename W::Tile;
+    constexpr int CC = W::CC, KS = W::KS, DT = W::DT, NB = W::NB, NCH = 2 * CC + DT / 2, MINE = NCH / 4;
     extern __shared__ float4 mx_lds[];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n16 = lane & 15;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t T = min(paso_T(a.paso), a.tcov), pos0 = paso_pos(a.paso);
-    const uint32_t G = a.nh / a.nkv, kvh = blockIdx.x, nrow = T * G;
-    // (long prompts: the blocks with the most keys first)
-    const uint32_t r0 = (TREE ? blockIdx.y : gridDim.y - 1 - blockIdx.y) * (16 * RG);
-    if (r0 >= nrow) return;
-    const uint32_t t_lo = r0 / G, t_hi = (min(r0 + 16 * RG, nrow) - 1) / G;
-    const uint32_t R = mx_slots(a.rows);
+    const W w(a);
+    if (w.b0 >= w.nrow) return;
+    const uint32_t lane = w.lane, g = w.g, n16 = w.n16, wave = w.wave;
+    const float scale = fabsf(a.scale) * MX_LOG2E;
     // ---- the rows' queries
     h8 qh[RG][KS], ql[RG][KS];
-    int qe[RG], lim[RG], low[RG];  // keys low < key <= lim
-    uint64_t mrow[RG];             // TREE: the row's mask words
-    bool alike = true;             // the lane's queries fit the f16 parts
-    auto q_at = [&](int r) __attribute__((always_inline)) {
-        const uint32_t rc = min(r0 + r * 16 + n16, nrow - 1);
-        return a.q + 4 * (((uint64_t)(rc / G) * a.nh + kvh * G + rc % G) * HD + 16 * g);
-    };
+    int qe[RG];
+    bool alike = true;  // the lane's fit the f16 parts
 #pragma unroll
     for (int r = 0; r < RG; r++) {
-        const uint32_t t = min(r0 + r * 16 + n16, nrow - 1) / G;
-        const uint64_t at = q_at(r);
-        float v[KS][8], mine = 0.0f, least = 3.4e38f;
+        const uint64_t at = w.query(r);
+        float v[KS][8], mine = 0.0f, least = 3.4e38f;  // the largest element, the least of the largest of 8 (not 0)
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            const float4 x = gload<float4>(at + (s >> 1) * 256 + (s & 1) * 32), y = gload<float4>(at + (s >> 1) * 256 + (s & 1) * 32 + 16);
-            const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            const float4 x = gload<float4>(at + (s >> 1) * 256 + (s & 1) * 32), z = gload<float4>(at + (s >> 1) * 256 + (s & 1) * 32 + 16);
+            const float f[8] = {x.x, x.y, x.z, x.w, z.x, z.y, z.z, z.w};
+            float eight = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float u = fabsf(w[i]);
-                v[s][i] = w[i];
-                mine = fmaxf(mine, u);
+                const float u = fabsf(f[i]);
+                v[s][i] = a.scale < 0.0f ? -f[i] : f[i];
+                eight = fmaxf(eight, u);
                 alike = alike & (u < __builtin_inff());  // (a NaN neither)
-                least = fminf(least, u == 0.0f ? 3.4e38f : u);
             }
+            mine = fmaxf(mine, eight);
+            least = fminf(least, eight == 0.0f ? 3.4e38f : eight);
         }
         float all = fmaxf(mine, bfly_f<4>(mine, lane));
         all = fmaxf(all, bfly_f<5>(all, lane));
         const int e = max((int)((__float_as_uint(all) >> 23) & 255) - 127, -110);
-        alike = alike & (least >= all * 0x1p-20f);
+        alike = alike & (least >= all * 0x1p-16f);
         qe[r] = e;
 #pragma unroll
         for (int s = 0; s < KS; s++)
@@ -318,379 +593,303 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
                 qh[r][s][i] = (_Float16)x;
                 ql[r][s][i] = (_Float16)(x - (float)qh[r][s][i]);
             }
-        uint32_t p = pos0 + t;
-        if constexpr (TREE) {
-            if (a.where) p = min(max(cptr<uint32_t>(a.where)[t], pos0), pos0 + T - 1);
-            mrow[r] = a.mask + 4ull * t * a.mw;
-        }
-        lim[r] = (int)p;
-        low[r] = a.swa && p >= a.swa ? (int)(p - a.swa) : -1;
     }
-    // ---- the key tiles: keys kbeg .. kend in slots first .. (ring: then 0 ..), whole tiles of 32 slots
-    const uint32_t last = TREE ? T - 1 : t_hi, early = TREE ? 0 : t_lo;
-    const uint32_t kend = a.cap ? pos0 + last + 1 : min(pos0 + last + 1, a.rows);
-    const uint32_t kbeg = a.swa && pos0 + early + 1 > a.swa ? min(pos0 + early + 1 - a.swa, kend) : 0;
-    const uint32_t first = a.cap ? kbeg % a.cap : kbeg, nkey = a.cap ? min(kend - kbeg, a.cap) : kend - kbeg;
-    const uint32_t end_a = a.cap ? min(first + nkey, a.cap) : first + nkey, end_b = first + nkey - end_a;
-    const uint32_t ta = nkey ? (end_a + 31) / 32 - first / 32 : 0, nt = ta + (end_b + 31) / 32;
-    const uint32_t per = (nt + a.nsplit - 1) / a.nsplit, i0 = blockIdx.z * per, i1 = min(nt, i0 + per);
-    const uint64_t planes = (uint64_t)a.nkv * R * HD, hk = (uint64_t)kvh * R * HD, hx = planes + (uint64_t)kvh * R * NB;
-    const __amdgpu_buffer_rsrc_t kr = kq_rsrc(a.kc + hk, (uint64_t)R * HD), vr = kq_rsrc(a.vc + hk, (uint64_t)R * HD);
-    const __amdgpu_buffer_rsrc_t kxr = kq_rsrc(a.kc + hx, (uint64_t)R * NB), vxr = kq_rsrc(a.vc + hx, (uint64_t)R * NB);
-
-    u32x4 kw[2][CC], vw[DT / 2];
+    const uint32_t i1 = w.i1;
+    const __amdgpu_buffer_rsrc_t kr = kq_rsrc(a.kc + w.hk, (uint64_t)w.R * HD), vr = kq_rsrc(a.vc + w.hk, (uint64_t)w.R * HD);
+    const __amdgpu_buffer_rsrc_t kxr = kq_rsrc(a.kc + w.hx, (uint64_t)w.R * NB), vxr = kq_rsrc(a.vc + w.hx, (uint64_t)w.R * NB);
     uint32_t kx[2], vx[2];  // the scales of the lane's key of each half, and of its 8 values' keys
-    struct Tile { uint32_t slot, lo, hi; int off; };  // slots lo .. hi of it hold keys slot + off
-    auto tile = [&](uint32_t i) __attribute__((always_inline)) {
-        Tile t;
-        if (i < ta) t = {(first / 32 + i) * 32, first, end_a, (int)(kbeg - first)};
-        else t = {(i - ta) * 32, 0, end_b, (int)(kbeg + a.cap - first)};
-        return t;
-    };
-    auto load_k = [&](uint32_t i) __attribute__((always_inline)) {
-        const uint32_t s = tile(i).slot, o = i < i1 ? s * HD + lane * 16 : QP_NOOFF;
+    auto load_kx = [&](uint32_t i) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const uint32_t x = i < i1 ? (s + h * 16 + n16) * NB : QP_NOOFF;
+            const uint32_t x = i < i1 ? (w.tile(i).slot + h * 16 + n16) * NB : QP_NOOFF;
             if constexpr (NB == 4) kx[h] = __builtin_amdgcn_raw_buffer_load_b32(kxr, x, 0, 0);
             else kx[h] = __builtin_amdgcn_raw_buffer_load_b16(kxr, x, 0, 0);
-#pragma unroll
-            for (int c = 0; c < CC; c++) kw[h][c] = __builtin_amdgcn_raw_buffer_load_b128(kr, o, (h * CC + c) * 1024, 0);
         }
     };
-    auto load_v = [&](uint32_t i) __attribute__((always_inline)) {
-        const uint32_t s = tile(i).slot, o = i < i1 ? s * HD + lane * 16 : QP_NOOFF;
-        const uint32_t x = i < i1 ? s * NB + (n16 * DT / 32) * 32 + g * 8 : QP_NOOFF;
-        const auto w = __builtin_amdgcn_raw_buffer_load_b64(vxr, x, 0, 0);
-        vx[0] = w[0];
-        vx[1] = w[1];
-#pragma unroll
-        for (int c = 0; c < DT / 2; c++) vw[c] = __builtin_amdgcn_raw_buffer_load_b128(vr, o, c * 1024, 0);
+    auto load_vx = [&](uint32_t i) __attribute__((always_inline)) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b64(vxr, i < i1 ? w.tile(i).slot * NB + (n16 * DT / 32) * 32 + g * 8 : QP_NOOFF, 0, 0);
+        vx[0] = x[0];
+        vx[1] = x[1];
     };
-    // slot k of the tile holds a key
-    auto held = [&](const Tile& t, uint32_t k) __attribute__((always_inline)) { return t.slot + k >= t.lo && t.slot + k < t.hi; };
-    // bits of the mask for the tile's 32 slots (drafted tokens only)
-    auto drafted = [&](const Tile& t, int r) __attribute__((always_inline)) -> uint32_t {
-        if constexpr (!TREE) return 0;
-        const int j = (int)t.slot + t.off - (int)pos0, w = j >> 5, sh = j & 31;
-        const uint32_t b0 = w >= 0 && w < (int)a.mw ? gload<uint32_t>(mrow[r] + 4ull * (uint32_t)w) : 0;
-        const uint32_t b1 = w + 1 >= 0 && w + 1 < (int)a.mw ? gload<uint32_t>(mrow[r] + 4ull * (uint32_t)(w + 1)) : 0;
-        return (uint32_t)((((uint64_t)b1 << 32) | b0) >> sh);
-    };
-    // row r sees the key in slot k of the tile
-    auto sees = [&](const Tile& t, int r, uint32_t k, uint32_t bits) __attribute__((always_inline)) {
-        const int key = (int)(t.slot + k) + t.off;
-        if constexpr (TREE) return held(t, k) & (key < (int)pos0 ? key > low[r] : ((bits >> k) & 1) != 0);
-        else return held(t, k) & (key <= lim[r]) & (key > low[r]);
-    };
-    // all slots hold keys that every row of the block sees
-    auto all_see = [&](const Tile& t) __attribute__((always_inline)) {
-        const int k0 = (int)t.slot + t.off;
-        return t.slot >= t.lo && t.slot + 32 <= t.hi && k0 + 31 <= (int)(pos0 + t_lo) - (TREE ? (int)t_lo + 1 : 0) &&
-               (!a.swa || k0 > (int)(pos0 + (TREE ? T - 1 : t_hi)) - (int)a.swa);
-    };
-
-    f32x4 o[RG][DT];
-    float m[RG], l[RG], p[RG][8], corr[RG], cs[RG];
+    MxState<HD, RG> st;
+    st.start();
+    float cs[RG];          // score = accumulator times cs, in units of log2
     int ek = -1, ev = -1;  // E of the keys and values, or -1: only zeros so far
 #pragma unroll
-    for (int r = 0; r < RG; r++) {
-        m[r] = -3.0e38f;
-        l[r] = 0.0f;
-        cs[r] = 0.0f;
+    for (int r = 0; r < RG; r++) cs[r] = 1.2e-38f;
+    auto wave_most = [&](int x) __attribute__((always_inline)) {  // of whole numbers below 2^24
+        return (int)__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max_v((float)x, lane))));
+    };
+    // The tile's scales made ready: those of slots without a key (which may hold anything) 0, E such that all fit; false
+    // where no E will do.  Lanes that hold the same scales look at a part of them each: byte g of their keys' (hd = 64:
+    // g % 2), bytes n16 % 4 of their values'.
+    auto ready = [&](const Tile& t) __attribute__((always_inline)) {
+        if (!w.full(t)) {
 #pragma unroll
-        for (int d = 0; d < DT; d++) o[r][d] = f32x4{0, 0, 0, 0};
-    }
-    // softmax of the lane's 8 keys of each of its rows: scores s times c in units of log2
-    auto softmax = [&](const Tile& t, bool whole, const f32x4 (&s)[RG][2], const float (&c)[RG]) __attribute__((always_inline)) {
+            for (int h = 0; h < 2; h++) {
+                kx[h] = w.held(t, h * 16 + n16) ? kx[h] : 0;
 #pragma unroll
-        for (int r = 0; r < RG; r++) {
-            const uint32_t bits = TREE && !whole ? drafted(t, r) : 0;
-            float x[8], mx = -3.0e38f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[j] = s[r][j >> 2][j & 3] * c[r];
-                if (!whole) x[j] = sees(t, r, (j >> 2) * 16 + 4 * g + (j & 3), bits) ? x[j] : -__builtin_inff();
-                mx = fmaxf(mx, x[j]);
+                for (int j = 0; j < 4; j++) vx[h] &= w.held(t, h * 16 + 4 * g + j) ? 0xffffffffu : ~(255u << (8 * j));
             }
-            mx = fmaxf(mx, bfly_f<4>(mx, lane));
-            mx = fmaxf(mx, bfly_f<5>(mx, lane));
-            const float mn = fmaxf(m[r], mx);
-            corr[r] = __builtin_amdgcn_exp2f(m[r] - mn);
-            m[r] = mn;
-            float sum = 0.0f;
+        }
+        const uint32_t ks = 8 * (g % NB), vs = 8 * (n16 & 3);
+        const int k0 = (kx[0] >> ks) & 255, k1 = (kx[1] >> ks) & 255;
+        int v0 = (vx[0] >> vs) & 255, v1 = (vx[1] >> vs) & 255;
+        const int kh = max(k0, k1);
+        int vh = max(v0, v1);
+        const int kl = min((k0 - 1) & 0xffff, (k1 - 1) & 0xffff) + 1;  // (0: no limit)
+        int vl = min((v0 - 1) & 0xffff, (v1 - 1) & 0xffff) + 1;
+        if (__all(kh <= ek && kl >= ek - 19 && vh <= ev && vl >= ev - 19)) return true;
+        // ---- seldom: the first tile, another E, blocks that are not finite
+        if (__any(vh == (int)MX_NAN) && !w.all_see(t, w.b_lo, w.b_hi)) {  // not every row sees every key: taken out
+            st.poison(w, t);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                p[r][j] = __builtin_amdgcn_exp2f(x[j] - mn);
-                sum += p[r][j];
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (((vx[i] >> (8 * j)) & 255) == MX_NAN) vx[i] &= ~(255u << (8 * j));
+            v0 = (vx[0] >> vs) & 255, v1 = (vx[1] >> vs) & 255;
+            vh = max(v0, v1);
+            vl = min((v0 - 1) & 0xffff, (v1 - 1) & 0xffff) + 1;
+        }
+        const int kmax = wave_most(kh), vmax = wave_most(vh), kmin = 65536 - wave_most(65536 - kl), vmin = 65536 - wave_most(65536 - vl);
+        if (max(kmax, vmax) == (int)MX_NAN || kmin < kmax - 19 || vmin < vmax - 19) return false;
+        if (kmax && (kmax > ek || kmin < ek - 19)) {
+            ek = min(min(kmax + 4, kmin + 19), 254);
+#pragma unroll
+            for (int r = 0; r < RG; r++) cs[r] = fmaxf(__builtin_ldexpf(scale, ek - 138 + qe[r] - 14), 1.2e-38f);
+        }
+        if (vmax && (vmax > ev || vmin < ev - 19)) {
+            const int e = min(min(vmax + 4, vmin + 19), 254);
+            if (ev >= 0) {
+                if (abs(e - ev) > 60) return false;  // (the sums could leave f32's range)
+#pragma unroll
+                for (int r = 0; r < RG; r++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) st.o[r][d][x] = __builtin_ldexpf(st.o[r][d][x], ev - e);
             }
-            l[r] = l[r] * corr[r] + sum;
+            ev = e;
+        }
+        return true;
+    };
+    auto pair = [&](uint32_t v, uint32_t i, uint32_t j) __attribute__((always_inline)) {  // bytes i and j of v
+        return __builtin_bit_cast(us2, __builtin_amdgcn_perm(0u, v, 0x0c000c00u | i | (j << 16)));
+    };
+    // 2^(x - E + 5) of two blocks as f16 (0 below the normal ones)
+    auto factor = [&](us2 x, int e) __attribute__((always_inline)) {
+        const uint16_t lo = (uint16_t)max(e - 20, 0), up = (uint16_t)max(20 - max(e, 0), 0);  // (exponent 20: 2^5)
+        return __builtin_bit_cast(h2, (us2)((__builtin_elementwise_sub_sat(x, us2{lo, lo}) + us2{up, up}) << us2{10, 10}));
+    };
+    const h2 k1152 = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    auto key_factors = [&](uint32_t x, int c, h2 (&s)[4], h2 (&off)[4]) __attribute__((always_inline)) {
+        const uint32_t at = 2 * c + (g >> 1);
+        s[0] = factor(pair(x, at, at), ek);
+        off[0] = s[0] * k1152;
+#pragma unroll
+        for (int i = 1; i < 4; i++) s[i] = s[0], off[i] = off[0];
+    };
+    auto value_factors = [&](h2 (&s)[4], h2 (&off)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            s[c] = factor(pair(vx[c >> 1], 2 * (c & 1), 2 * (c & 1) + 1), ev);
+            off[c] = s[c] * k1152;
         }
     };
-    auto rescale = [&]() __attribute__((always_inline)) {
-        bool same = true;
+    // eight bytes q + 128 as f16 times the factors s (of two bytes each), off = -1152 s
+    auto unpack8 = [&](uint32_t w0, uint32_t w1, const h2 (&s)[4], const h2 (&off)[4]) __attribute__((always_inline)) {
+        h8 v;
 #pragma unroll
-        for (int r = 0; r < RG; r++) same = same && corr[r] == 1.0f;
-        if (__all(same)) return;
+        for (int c = 0; c < 4; c++) {
+            const h2 u = __builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(0x64646464u, c < 2 ? w0 : w1, c & 1 ? 0x04030402u : 0x04010400u)), s[c], off[c]);
+            v[2 * c] = u[0];
+            v[2 * c + 1] = u[1];
+        }
+        return v;
+    };
+    h8 ph[RG], pl[RG];
+    auto split_p = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < RG; r++)
 #pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) o[r][d][x] *= corr[r];
+            for (int j = 0; j < 8; j++) {
+                ph[r][j] = (_Float16)(st.p[r][j] * MX_UP);
+                pl[r][j] = (_Float16)fmaf(st.p[r][j], MX_UP, -(float)ph[r][j]);
+            }
     };
-    // the scales of slots without a key: 0 (they may hold anything)
-    auto clear = [&](const Tile& t) __attribute__((always_inline)) {
-        if (t.slot >= t.lo && t.slot + 32 <= t.hi) return;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            kx[h] = held(t, h * 16 + n16) ? kx[h] : 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) vx[h] &= held(t, h * 16 + 4 * g + j) ? 0xffffffffu : ~(255u << (8 * j));
-        }
-    };
-    // A value that is not finite reaches the rows that see its key, and no others: their channels become NaN here (the
-    // lane's own, which are of one block), the scale 0.
-    auto poison = [&](const Tile& t) __attribute__((always_inline)) {
-        uint32_t bad = 0;
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) bad |= ((vx[i] >> (8 * j)) & 255) == MX_NAN ? 1u : 0u;
-        if (!__any(bad != 0)) return;
-        const uint64_t xs = a.vc + hx + (uint64_t)t.slot * NB + (DT * 4 * g / 32) * 32;
+    auto scores = [&](f32x4 (&s)[RG][2], int h, int c, h8 k) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < RG; r++) {
-            const uint32_t bits = drafted(t, r);
-            bool nan = false;
-            for (uint32_t i = 0; i < 32; i++) {  // byte i: lane group i / 8, value i % 8
-                const uint32_t k = ((i >> 2) & 1) * 16 + 4 * (i >> 3) + (i & 3);
-                nan |= sees(t, r, k, bits) && gload<uint8_t>(xs + i) == MX_NAN;
-            }
-            if (nan)
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[r][d] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            s[r][h] = mx_mfma(k, qh[r][c], c ? s[r][h] : f32x4{0, 0, 0, 0});
+            s[r][h] = mx_mfma(k, ql[r][c], s[r][h]);
         }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (((vx[i] >> (8 * j)) & 255) == MX_NAN) vx[i] &= ~(255u << (8 * j));
     };
-    // E for scales up to the lanes' b: 4 above the largest; -1: all 0
-    auto widest = [&](int b) __attribute__((always_inline)) {
-        const int x = (int)__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max_v(b == (int)MX_NAN ? 0.0f : (float)b, lane))));
-        return x ? min(x + 4, 254) : -1;
-    };
-    auto pair = [&](uint32_t w, int i) __attribute__((always_inline)) {  // bytes 2 i and 2 i + 1 of w
-        return __builtin_bit_cast(us2, __builtin_amdgcn_perm(0u, w, i ? 0x0c030c02u : 0x0c010c00u));
-    };
-    // two bytes q + 128 of w (sel) as f16 times the scales s, off = -1152 s
-    auto unpack = [&](uint32_t w, uint32_t sel, h2 s, h2 off) __attribute__((always_inline)) {
-        return __builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(0x64646464u, w, sel)), s, off);
-    };
-    const h2 k1152 = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    uint32_t i = i0 + wave;
-    load_k(i);
-    load_v(i);
-    if (__all(alike)) {
-        for (; i < i1; i += 4) {
-            const Tile t = tile(i);
-            const bool whole = all_see(t);
-            clear(t);
-            if (!whole) poison(t);
-            us2 hi = {0, 0}, lo = {0xffff, 0xffff};  // the largest scale, and the smallest that is not 0, less 1
-            auto note = [&](us2 b) __attribute__((always_inline)) {
-                hi = __builtin_elementwise_max(hi, b);
-                lo = __builtin_elementwise_min(lo, (us2)(b - us2{1, 1}));
-            };
-            note(pair(kx[0], 0)), note(pair(kx[1], 0));
-            if constexpr (NB == 4) note(pair(kx[0], 1)), note(pair(kx[1], 1));
-            const int khi = max(hi[0], hi[1]), klo = min(lo[0], lo[1]);
-            hi = us2{0, 0}, lo = us2{0xffff, 0xffff};
+    auto outputs = [&](int d, h8 v) __attribute__((always_inline)) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) note(pair(vx[c >> 1], c & 1));
-            const int vhi = max(hi[0], hi[1]), vlo = min(lo[0], lo[1]);
-            // the wavefront's E: from its first tile that is not all zeros
-            if (ek < 0 && (ek = widest(khi)) >= 0) {
+        for (int r = 0; r < RG; r++) {
+            st.o[r][d] = mx_mfma(v, ph[r], st.o[r][d]);
+            st.o[r][d] = mx_mfma(v, pl[r], st.o[r][d]);
+        }
+    };
+    bool ok = __syncthreads_and(alike) != 0;
+    if constexpr (!WIDE) {
+        // the tiles are dealt to the wavefronts, each with a state of its own
+        u32x4 kw[2 * CC], vw[DT / 2];
+        auto load_k = [&](uint32_t i) __attribute__((always_inline)) {
+            const uint32_t o = i < i1 ? w.tile(i).slot * HD + lane * 16 : QP_NOOFF;
+            load_kx(i);
 #pragma unroll
-                for (int r = 0; r < RG; r++) cs[r] = __builtin_ldexpf(a.scale * MX_LOG2E, ek - 138 + qe[r] - 14);
+            for (int c = 0; c < 2 * CC; c++) kw[c] = __builtin_amdgcn_raw_buffer_load_b128(kr, o, c * 1024, 0);
+        };
+        auto load_v = [&](uint32_t i) __attribute__((always_inline)) {
+            const uint32_t o = i < i1 ? w.tile(i).slot * HD + lane * 16 : QP_NOOFF;
+            load_vx(i);
+#pragma unroll
+            for (int c = 0; c < DT / 2; c++) vw[c] = __builtin_amdgcn_raw_buffer_load_b128(vr, o, c * 1024, 0);
+        };
+        uint32_t i = w.i0 + wave;
+        load_k(i);
+        load_v(i);
+        for (; ok && i < i1; i += 4) {
+            const Tile t = w.tile(i);
+            if (!ready(t)) {
+                ok = false;
+                break;
             }
-            if (ev < 0) ev = widest(vhi);
-            if (!__all(khi <= max(ek, 0) && klo + 1 >= ek - 19 && vhi <= max(ev, 0) && vlo + 1 >= ev - 19)) break;
-            // ---- S^T = K Q^T
-            const us2 bk = {(uint16_t)max(ek - 20, 0), (uint16_t)max(ek - 20, 0)};  // (exponent 20: 2^5)
-            const us2 dk = {(uint16_t)max(20 - max(ek, 0), 0), (uint16_t)max(20 - max(ek, 0), 0)};
             f32x4 s[RG][2];
+            h2 f[4], off[4];
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int c = 0; c < CC; c++) {
-                    const uint32_t at = 2 * c + (g >> 1);
-                    const us2 b = __builtin_bit_cast(us2, __builtin_amdgcn_perm(0u, kx[h], 0x0c000c00u | at | (at << 16)));
-                    const h2 sc = __builtin_bit_cast(h2, (us2)((__builtin_elementwise_sub_sat(b, bk) + dk) << us2{10, 10}));
-                    const h2 off = sc * k1152;
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        h8 k;
-#pragma unroll
-                        for (int y = 0; y < 4; y++) {
-                            const h2 v = unpack(kw[h][c][2 * x + (y >> 1)], y & 1 ? 0x04030402u : 0x04010400u, sc, off);
-                            k[2 * y] = v[0];
-                            k[2 * y + 1] = v[1];
-                        }
-#pragma unroll
-                        for (int r = 0; r < RG; r++) {
-                            s[r][h] = mx_mfma(k, qh[r][2 * c + x], c + x ? s[r][h] : f32x4{0, 0, 0, 0});
-                            s[r][h] = mx_mfma(k, ql[r][2 * c + x], s[r][h]);
-                        }
-                    }
+                    key_factors(kx[h], c, f, off);
+                    scores(s, h, 2 * c, unpack8(kw[h * CC + c][0], kw[h * CC + c][1], f, off));
+                    scores(s, h, 2 * c + 1, unpack8(kw[h * CC + c][2], kw[h * CC + c][3], f, off));
                 }
             load_k(i + 4);
-            softmax(t, whole, s, cs);
-            rescale();
-            // ---- O^T += V^T P^T
-            h8 ph[RG], pl[RG];
+            st.softmax(w, t, s, cs);
+            split_p();
+            value_factors(f, off);
 #pragma unroll
-            for (int r = 0; r < RG; r++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float x = p[r][j] * 0x1p15f;  // (so that small probabilities keep their low parts)
-                    ph[r][j] = (_Float16)x;
-                    pl[r][j] = (_Float16)(x - (float)ph[r][j]);
-                }
-            const us2 bv = {(uint16_t)max(ev - 20, 0), (uint16_t)max(ev - 20, 0)};
-            const us2 dv = {(uint16_t)max(20 - max(ev, 0), 0), (uint16_t)max(20 - max(ev, 0), 0)};
-            h2 sv[4], ov[4];
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                sv[c] = __builtin_bit_cast(h2, (us2)((__builtin_elementwise_sub_sat(pair(vx[c >> 1], c & 1), bv) + dv) << us2{10, 10}));
-                ov[c] = sv[c] * k1152;
-            }
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                h8 v;
-#pragma unroll
-                for (int y = 0; y < 4; y++) {
-                    const h2 u = unpack(vw[d >> 1][2 * (d & 1) + (y >> 1)], y & 1 ? 0x04030402u : 0x04010400u, sv[y], ov[y]);
-                    v[2 * y] = u[0];
-                    v[2 * y + 1] = u[1];
-                }
-#pragma unroll
-                for (int r = 0; r < RG; r++) {
-                    o[r][d] = mx_mfma(v, ph[r], o[r][d]);
-                    o[r][d] = mx_mfma(v, pl[r], o[r][d]);
-                }
-            }
+            for (int d = 0; d < DT; d++) outputs(d, unpack8(vw[d >> 1][2 * (d & 1)], vw[d >> 1][2 * (d & 1) + 1], f, off));
             load_v(i + 4);
         }
-    }
-    int back = max(ev, 0) - 153;  // o times 2^back: the outputs
-    if (i < i1) {  // the other tiles in f32
+        ok = __syncthreads_and(ok) != 0;
+    } else {
+        // every wavefront takes every tile, of which each unpacks a quarter to f16 in LDS (two buffers): chunk c of a tile
+        // (1 KB: of K below 2 CC, then of V) is the wavefront's where c % 4 == wave
+        h8* lds = reinterpret_cast<h8*>(mx_lds);  // [buffer][chunk][half of the lane's bytes][lane]
+        u32x4 raw[MINE];
+        auto load = [&](uint32_t j) __attribute__((always_inline)) {
+            const uint32_t at = j < i1 ? w.tile(j).slot * HD + lane * 16 : QP_NOOFF;
+            load_kx(j);
+            load_vx(j);
 #pragma unroll
-        for (int r = 0; r < RG; r++)
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) o[r][d][x] = __builtin_ldexpf(o[r][d][x], back);
-        back = 0;
-        float c[RG];
-#pragma unroll
-        for (int r = 0; r < RG; r++) c[r] = a.scale * MX_LOG2E;
-        for (; i < i1; i += 4) {
-            const Tile t = tile(i);
-            const bool whole = all_see(t);
-            clear(t);
-            if (!whole) poison(t);
-            f32x4 s[RG][2];
-#pragma unroll
-            for (int r = 0; r < RG; r++) {
-                const uint64_t at = q_at(r);
-                s[r][0] = s[r][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int cc = 0; cc < CC; cc++)
-#pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        const float q = gload<float>(at + cc * 256 + 4 * x);
-#pragma unroll
-                        for (int h = 0; h < 2; h++)
-                            s[r][h] = mx_mfma(mx_value((kw[h][cc][x >> 2] >> (8 * (x & 3))) & 255, (kx[h] >> (8 * (2 * cc + (g >> 1)))) & 255), q, s[r][h]);
-                    }
+            for (int u = 0; u < MINE; u++) {
+                const uint32_t c = wave + 4 * u;
+                raw[u] = c < 2 * CC ? __builtin_amdgcn_raw_buffer_load_b128(kr, at, c * 1024, 0)
+                                    : __builtin_amdgcn_raw_buffer_load_b128(vr, at, (c - 2 * CC) * 1024, 0);
             }
-            load_k(i + 4);
-            softmax(t, whole, s, c);
-            rescale();
+        };
+        auto stage = [&](uint32_t j) __attribute__((always_inline)) {
 #pragma unroll
-            for (int d = 0; d < DT; d++)
+            for (int u = 0; u < MINE; u++) {
+                const uint32_t c = wave + 4 * u;
+                h2 f[4], off[4];
+                if (c < 2 * CC) key_factors(c / CC ? kx[1] : kx[0], c % CC, f, off);
+                else value_factors(f, off);
+                h8* to = lds + ((j & 1) * NCH + c) * 128 + lane;
+                to[0] = unpack8(raw[u][0], raw[u][1], f, off);
+                to[64] = unpack8(raw[u][2], raw[u][3], f, off);
+            }
+        };
+        uint32_t i = w.i0;
+        if (ok && i < i1) {
+            load(i);
+            ok = ready(w.tile(i));
+            if (ok) stage(i);
+            load(i + 1);
+            __syncthreads();
+            while (ok) {
+                const Tile t = w.tile(i);
+                if (w.wanted(t)) {
+                    const h8* from = lds + (i & 1) * NCH * 128 + lane;
+                    f32x4 s[RG][2];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float v = mx_value((vw[d >> 1][2 * (d & 1) + (j >> 2)] >> (8 * (j & 3))) & 255, (vx[j >> 2] >> (8 * (j & 3))) & 255);
+                    for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int r = 0; r < RG; r++) o[r][d] = mx_mfma(v, p[r][j], o[r][d]);
+                        for (int c = 0; c < KS; c++) scores(s, h, c, from[(h * KS + c) * 64]);
+                    st.softmax(w, t, s, cs);
+                    split_p();
+#pragma unroll
+                    for (int d = 0; d < DT; d++) outputs(d, from[(2 * KS + d) * 64]);
                 }
-            load_v(i + 4);
-        }
-    }
-    // ---- the four wavefronts' states meet: [wave][row][HD + 4], then [wave][row] (m, l)
-    constexpr int LD = HD + 4;
-    float* ol = reinterpret_cast<float*>(mx_lds);
-    float* ml = ol + 4 * RG * 16 * LD;
-#pragma unroll
-    for (int r = 0; r < RG; r++) {
-        float lt = l[r];
-        lt += bfly_f<4>(lt, lane);
-        lt += bfly_f<5>(lt, lane);
-        const uint32_t at = wave * RG * 16 + r * 16 + n16;
-        if (g == 0) {
-            ml[2 * at] = m[r];
-            ml[2 * at + 1] = lt;
-        }
-        // dimensions DT * (4 g + x) + d of the row
-#pragma unroll
-        for (int x = 0; x < 4; x++)
-#pragma unroll
-            for (int d = 0; d < DT; d += 4)
-                *reinterpret_cast<float4*>(ol + at * LD + DT * (4 * g + x) + d) =
-                    make_float4(__builtin_ldexpf(o[r][d][x], back), __builtin_ldexpf(o[r][d + 1][x], back),
-                                __builtin_ldexpf(o[r][d + 2][x], back), __builtin_ldexpf(o[r][d + 3][x], back));
-    }
-    __syncthreads();
-    for (uint32_t k = tid; k < RG * 16 * (HD / 4); k += 256) {
-        const uint32_t lr = k / (HD / 4), c = k % (HD / 4), row = r0 + lr;
-        if (row >= nrow) continue;
-        float M = -3.0e38f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) M = fmaxf(M, ml[2 * (w * RG * 16 + lr)]);
-        float L = 0.0f;
-        float4 s = make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const uint32_t at = w * RG * 16 + lr;
-            const float lw = ml[2 * at + 1];
-            if (lw != 0.0f) {
-                const float f = __builtin_amdgcn_exp2f(ml[2 * at] - M);
-                const float4 v = *reinterpret_cast<const float4*>(ol + at * LD + 4 * c);
-                L += lw * f;
-                s = make_float4(s.x + v.x * f, s.y + v.y * f, s.z + v.z * f, s.w + v.w * f);
+                if (++i >= i1) break;
+                ok = ready(w.tile(i));  // (the same in all wavefronts: they see the same scales)
+                if (ok) stage(i);
+                load(i + 1);
+                __syncthreads();
             }
         }
-        const uint32_t t = row / G, h = kvh * G + row % G;
-        const uint64_t at = (uint64_t)t * a.nh + h;
-        if (a.nsplit == 1) {
-            const float4 z = L == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(s.x / L, s.y / L, s.z / L, s.w / L);
-            gstore<float4>(a.o + 4 * (at * HD + 4 * c), z);
-        } else {
-            gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + 4 * c), s);
-            if (c == 0) gstore<float2>(a.part_ml + 8 * (at * a.nsplit + blockIdx.z), make_float2(M, L));
+    }
+    if (!ok) {
+        attn_mx8_f32<HD, RG, TREE, WIDE>((const __attribute__((address_space(4))) QpAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr());
+        return;
+    }
+    const int back = max(ev, 0) - 138 - 12;  // o times 2^back: the outputs
+    st.sum_l(lane);
+    if constexpr (WIDE) {
+        st.put_all(w, back);
+    } else {
+        // ---- the four wavefronts' states meet: [wave][row][HD + 4], then [wave][row] (m, l)
+        constexpr int LD = HD + 4;
+        float* ol = reinterpret_cast<float*>(mx_lds);
+        float* ml = ol + 4 * RG * 16 * LD;
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            const uint32_t at = wave * RG * 16 + r * 16 + n16;
+            if (g == 0) {
+                ml[2 * at] = st.m[r];
+                ml[2 * at + 1] = st.l[r];
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+#pragma unroll
+                for (int d = 0; d < DT; d += 4) *reinterpret_cast<float4*>(ol + at * LD + DT * (4 * g + x) + d) = st.out4(r, x, d, back);
+        }
+        __syncthreads();
+        for (uint32_t k = threadIdx.x; k < RG * 16 * (HD / 4); k += 256) {
+            const uint32_t lr = k / (HD / 4), c = 4 * (k % (HD / 4)), row = w.r0 + lr;
+            if (row >= w.nrow) continue;
+            float M = -3.0e38f;
+#pragma unroll
+            for (int v = 0; v < 4; v++) M = fmaxf(M, ml[2 * (v * RG * 16 + lr)]);
+            float L = 0.0f;
+            float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const uint32_t at = v * RG * 16 + lr;
+                const float lw = ml[2 * at + 1];
+                if (lw != 0.0f) {
+                    const float f = __builtin_amdgcn_exp2f(ml[2 * at] - M);
+                    const float4 x = *reinterpret_cast<const float4*>(ol + at * LD + c);
+                    L += lw * f;
+                    s = make_float4(s.x + x.x * f, s.y + x.y * f, s.z + x.z * f, s.w + x.w * f);
+                }
+            }
+            w.put(row, c, s, M, L);
         }
     }
 }
 
 #define ATTN_MX8(HD, NAME, TREE)                                                                                      \
     KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void qp_attn_mx8_h##HD##_##NAME##_r1(       \
-        QpAttnArgs a) { attn_mx8_body<HD, 1, TREE>(a); }                                                              \
+        QpAttnArgs a) { attn_mx8_body<HD, 1, TREE, false>(a); }                                                       \
     KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void qp_attn_mx8_h##HD##_##NAME##_r2(       \
-        QpAttnArgs a) { attn_mx8_body<HD, 2, TREE>(a); }
+        QpAttnArgs a) { attn_mx8_body<HD, 2, TREE, false>(a); }                                                       \
+    KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void qp_attn_mx8_h##HD##_##NAME##_wide(     \
+        QpAttnArgs a) { attn_mx8_body<HD, 2, TREE, true>(a); }
 ATTN_MX8(64, causal, false) ATTN_MX8(128, causal, false) ATTN_MX8(64, tree, true) ATTN_MX8(128, tree, true)
 
 // The shares' partial states of each (query, head) row -> o, in their order: grid rows, hd threads (at most 64 shares).

@@ -1165,9 +1165,13 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     if (int e = need_room(a.q, qb, op, "q")) return e;
     if (int e = need_room(a.o, qb, op, "the output")) return e;
     const uint64_t nrow = (uint64_t)T * G;
-    const uint32_t RG = nrow > 16 ? 2 : 1;
-    if (cdiv(nrow, 16 * RG) > 65535) return fail(QP_E_ARG, "%s: %u tokens in one call", op, T);
-    const uint32_t yb = cdiv(nrow, 16 * RG);
+#ifndef MX_WIDE_FROM
+#define MX_WIDE_FROM 65
+#endif
+    const bool wide = fmt == QP_KV_MX8 && nrow >= MX_WIDE_FROM;
+    const uint32_t RG = nrow > 16 ? 2 : 1, block = wide ? 128 : 16 * RG;
+    if (cdiv(nrow, block) > 65535) return fail(QP_E_ARG, "%s: %u tokens in one call", op, T);
+    const uint32_t yb = cdiv(nrow, block);
     const uint64_t per = (uint64_t)T * a.nh * (4 * a.hd + 8);  // bytes of one share's partial states
     if (ns > 64) return fail(QP_E_ARG, "%s: %u shares of the keys (at most 64)", op, ns);
     if (ns > 1) {
@@ -1195,8 +1199,9 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
                                     {{K_attn_mx8_h64_tree_r1, K_attn_mx8_h64_tree_r2}, {K_attn_mx8_h128_tree_r1, K_attn_mx8_h128_tree_r2}}};
     static const Kid kt[2][2][2] = {{{K_attn_t_h64_f32_r1, K_attn_t_h64_f32_r2}, {K_attn_t_h128_f32_r1, K_attn_t_h128_f32_r2}},
                                     {{K_attn_t_h64_f16_r1, K_attn_t_h64_f16_r2}, {K_attn_t_h128_f16_r1, K_attn_t_h128_f16_r2}}};
-    const Kid k = fmt == QP_KV_MX8 ? k8[tree][a.hd == 128][RG == 2] : kt[fmt][a.hd == 128][RG == 2];
-    const uint32_t lds = 4 * RG * 16 * (a.hd + 4) * 4 + 4 * RG * 16 * 8;
+    static const Kid kw[2][2] = {{K_attn_mx8_h64_causal_wide, K_attn_mx8_h128_causal_wide}, {K_attn_mx8_h64_tree_wide, K_attn_mx8_h128_tree_wide}};
+    const Kid k = wide ? kw[tree][a.hd == 128] : fmt == QP_KV_MX8 ? k8[tree][a.hd == 128][RG == 2] : kt[fmt][a.hd == 128][RG == 2];
+    const uint32_t lds = wide ? 2 * 128 * a.hd : 4 * RG * 16 * (a.hd + 4) * 4 + 4 * RG * 16 * 8;
     if (int e = launch(k, a.nkv, yb, ns, 256, lds, a)) return e;
     return ns == 1 ? 0 : launch(K_attn_mx8_comb, T * a.nh, 1, 1, a.hd, 0, a);
 }
