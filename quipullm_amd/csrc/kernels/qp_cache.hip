@@ -266,12 +266,13 @@ constexpr float MX_LOG2E = 1.4426950408889634f;
 // computes its rows with the f32 matrix instruction instead (attn_mx8_f32, some ten times slower).  So no row loses bits to a
 // key that it does not see.
 //
-// The softmax's reference m of a row follows its largest score only when a tile passes it by 2^MX_LAG: until then
-// probabilities of up to 2^MX_LAG are summed as they are, and no wavefront exchanges maxima or rescales its outputs.
-constexpr float MX_LAG = 3.0f, MX_UP = 0x1p12f;  // probabilities times MX_UP: below 2^15
+// Probabilities are 2^(s - m) with a reference m of the row that lies MX_UP below its largest score, so that their f16 parts
+// stay normal.  m follows the largest score only when a tile passes it by MX_LAG: until then probabilities of up to
+// 2^(MX_UP + MX_LAG) are summed as they are, and no wavefront exchanges maxima or rescales its outputs.
+constexpr float MX_LAG = 5.0f, MX_UP = 10.0f;
 
-// What a wavefront works on.  WIDE: a workgroup takes 64 RG (query, head) rows of one KV head, 16 RG for each of its four
-// wavefronts, and all of them take all tiles of its share of the keys; else all have the same 16 RG rows.
+// What a wavefront works on.  WIDE: a workgroup takes 128 RG (query, head) rows of one KV head, 16 RG for each of its eight
+// wavefronts, and all of them take all tiles of its share of the keys; else its four have the same 16 RG rows.
 template <int HD, int RG, bool TREE, bool WIDE>
 struct MxWork {
     static constexpr int CC = HD / 64, KS = HD / 32, DT = HD / 16, NB = HD / 32;
@@ -280,21 +281,21 @@ struct MxWork {
     uint32_t b0, b_lo, b_hi, r0, t_lo, t_hi;  // the workgroup's rows and their tokens, the wavefront's
     uint32_t kbeg, first, end_a, end_b, ta, i0, i1;
     uint64_t hk, hx;                          // the head's bytes and scales in a cache
-    int lim[RG], low[RG];                     // the lane's rows see keys low < key <= lim
-    uint64_t mrow[RG];                        // TREE: and the drafted ones of their mask words
+    int lim[RG];                              // the lane's rows' positions: they see keys lim - swa < key <= lim,
+    uint32_t word[RG];                        // TREE: those below pos0, and the drafted ones of their mask words
     const QpAttnArgs& a;
 
     QP_DEV MxWork(const QpAttnArgs& args) : a(args) {
         lane = threadIdx.x & 63, g = lane >> 4, n16 = lane & 15;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        T = min(paso_T(a.paso), a.tcov), pos0 = paso_pos(a.paso);
+        T = min(__builtin_amdgcn_readfirstlane(paso_T(a.paso)), a.tcov), pos0 = __builtin_amdgcn_readfirstlane(paso_pos(a.paso));
         G = a.nh / a.nkv, kvh = blockIdx.x, nrow = T * G, R = mx_slots(a.rows);
         // long prompts: the blocks with the most keys first, then those with the fewest on (two workgroups share a CU)
         const uint32_t y = blockIdx.y, ny = gridDim.y, blk = TREE ? y : y < (ny + 1) / 2 ? ny - 1 - y : y - (ny + 1) / 2;
-        b0 = blk * (WIDE ? 64 * RG : 16 * RG);
+        b0 = blk * (WIDE ? 128 * RG : 16 * RG);
         r0 = b0 + (WIDE ? wave * 16 * RG : 0);
         if (b0 >= nrow) return;
-        b_lo = b0 / G, b_hi = (min(b0 + (WIDE ? 64 * RG : 16 * RG), nrow) - 1) / G;
+        b_lo = b0 / G, b_hi = (min(b0 + (WIDE ? 128 * RG : 16 * RG), nrow) - 1) / G;
         t_lo = min(r0, nrow - 1) / G, t_hi = (min(r0 + 16 * RG, nrow) - 1) / G;
 #pragma unroll
         for (int r = 0; r < RG; r++) {
@@ -302,10 +303,9 @@ struct MxWork {
             uint32_t p = pos0 + t;
             if constexpr (TREE) {
                 if (a.where) p = min(max(cptr<uint32_t>(a.where)[t], pos0), pos0 + T - 1);
-                mrow[r] = a.mask + 4ull * t * a.mw;
+                word[r] = t * a.mw;
             }
             lim[r] = (int)p;
-            low[r] = a.swa && p >= a.swa ? (int)(p - a.swa) : -1;
         }
         // the key tiles: keys kbeg .. kend in slots first .. (ring: then 0 ..), whole tiles of 32 slots
         const uint32_t last = TREE ? T - 1 : b_hi, early = TREE ? 0 : b_lo;
@@ -336,15 +336,16 @@ struct MxWork {
     QP_DEV uint32_t drafted(const Tile& t, int r) const {
         if constexpr (!TREE) return 0;
         const int j = (int)t.slot + t.off - (int)pos0, w = j >> 5, sh = j & 31;
-        const uint32_t w0 = w >= 0 && w < (int)a.mw ? gload<uint32_t>(mrow[r] + 4ull * (uint32_t)w) : 0;
-        const uint32_t w1 = w + 1 >= 0 && w + 1 < (int)a.mw ? gload<uint32_t>(mrow[r] + 4ull * (uint32_t)(w + 1)) : 0;
+        const uint32_t w0 = w >= 0 && w < (int)a.mw ? gload<uint32_t>(a.mask + 4ull * (word[r] + (uint32_t)w)) : 0;
+        const uint32_t w1 = w + 1 >= 0 && w + 1 < (int)a.mw ? gload<uint32_t>(a.mask + 4ull * (word[r] + (uint32_t)(w + 1))) : 0;
         return (uint32_t)((((uint64_t)w1 << 32) | w0) >> sh);
     }
     // the lane's row sees the key in slot k of the tile
     QP_DEV bool sees(const Tile& t, int r, uint32_t k, uint32_t bits) const {
         const int key = (int)(t.slot + k) + t.off;
-        if constexpr (TREE) return held(t, k) & (key < (int)pos0 ? key > low[r] : ((bits >> k) & 1) != 0);
-        else return held(t, k) & (key <= lim[r]) & (key > low[r]);
+        const bool in = !a.swa || key > lim[r] - (int)a.swa;
+        if constexpr (TREE) return held(t, k) & (key < (int)pos0 ? in : ((bits >> k) & 1) != 0);
+        else return held(t, k) & (key <= lim[r]) & in;
     }
     // all slots hold keys that all rows of tokens lo .. hi see
     QP_DEV bool all_see(const Tile& t, uint32_t lo, uint32_t hi) const {
@@ -360,7 +361,8 @@ struct MxWork {
     QP_DEV void put(uint32_t row, uint32_t c, float4 s, float m, float l) const {
         const uint64_t at = (uint64_t)(row / G) * a.nh + kvh * G + row % G;
         if (a.nsplit == 1) {
-            gstore<float4>(a.o + 4 * (at * HD + c), l == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(s.x / l, s.y / l, s.z / l, s.w / l));
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;  // (l = 0: no key seen, and s = 0)
+            gstore<float4>(a.o + 4 * (at * HD + c), make_float4(s.x * f, s.y * f, s.z * f, s.w * f));
         } else {
             gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + c), s);
             if (c == 0) gstore<float2>(a.part_ml + 8 * (at * a.nsplit + blockIdx.z), make_float2(m, l));
@@ -386,9 +388,12 @@ struct MxState {
             for (int d = 0; d < DT; d++) o[r][d] = f32x4{0, 0, 0, 0};
         }
     }
-    // The probabilities p of the lane's 8 keys of each row, from the accumulators s (scores: times c, in units of log2).
+    // Accumulators s of the lane's 8 keys of each row (scores: times unit, in units of log2): those of keys that the row does not
+    // see become -inf, and the row's reference m follows them.  c: what s is to be multiplied by from now on.
     template <class W>
-    QP_DEV void softmax(const W& w, const typename W::Tile& t, f32x4 (&s)[RG][2], const float (&c)[RG]) {
+    QP_DEV void follow(const W& w, const typename W::Tile& t, f32x4 (&s)[RG][2], const float (&unit)[RG], float (&c)[RG]) {
+#pragma unroll
+        for (int r = 0; r < RG; r++) c[r] = unit[r];
         if (!w.all_see(t, w.t_lo, w.t_hi)) {
 #pragma unroll
             for (int r = 0; r < RG; r++) {
@@ -405,7 +410,7 @@ struct MxState {
             mx[r] = s[r][0][0];
 #pragma unroll
             for (int j = 1; j < 8; j++) mx[r] = fmaxf(mx[r], s[r][j >> 2][j & 3]);
-            past = past | (mx[r] * c[r] > m[r] + MX_LAG);
+            past = past | (mx[r] * c[r] > m[r] + (MX_UP + MX_LAG));
         }
         if (__any(past)) {
             bool b = false;
@@ -413,7 +418,7 @@ struct MxState {
             for (int r = 0; r < RG; r++) {
                 mx[r] = fmaxf(mx[r], bfly_f<4>(mx[r], w.lane));
                 mx[r] = fmaxf(mx[r], bfly_f<5>(mx[r], w.lane));
-                const float mn = fmaxf(m[r], mx[r] * c[r]), f = __builtin_amdgcn_exp2f(m[r] - mn);
+                const float mn = fmaxf(m[r], mx[r] * c[r] - MX_UP), f = __builtin_amdgcn_exp2f(m[r] - mn);
                 m[r] = mn;
                 l[r] *= f;
 #pragma unroll
@@ -424,25 +429,27 @@ struct MxState {
             }
             far = __any(b) != 0;
         }
-        if (far) {  // (s c - m in one rounding could be as large as half of m's last place)
+        if (far) {  // (s c - m in one rounding could be as large as half of m's last place: s c first)
 #pragma unroll
-            for (int r = 0; r < RG; r++)
+            for (int r = 0; r < RG; r++) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-#pragma clang fp contract(off)
-                    const float x = s[r][j >> 2][j & 3] * c[r];
-                    p[r][j] = __builtin_amdgcn_exp2f(x - m[r]);
-                }
-        } else {
-#pragma unroll
-            for (int r = 0; r < RG; r++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) p[r][j] = __builtin_amdgcn_exp2f(fmaf(s[r][j >> 2][j & 3], c[r], -m[r]));
+                for (int j = 0; j < 8; j++) s[r][j >> 2][j & 3] *= c[r];
+                c[r] = 1.0f;
+            }
         }
+    }
+    // Their probabilities p: of keys j and j + 1 of row r.
+    QP_DEV void weigh2(const f32x4 (&s)[RG][2], const float (&c)[RG], int r, int j) {
+        p[r][j] = __builtin_amdgcn_exp2f(fmaf(s[r][j >> 2][j & 3], c[r], -m[r]));
+        p[r][j + 1] = __builtin_amdgcn_exp2f(fmaf(s[r][j >> 2][(j & 3) + 1], c[r], -m[r]));
+        l[r] += p[r][j];
+        l[r] += p[r][j + 1];
+    }
+    QP_DEV void weigh(const f32x4 (&s)[RG][2], const float (&c)[RG]) {
 #pragma unroll
         for (int r = 0; r < RG; r++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) l[r] += p[r][j];
+            for (int j = 0; j < 8; j += 2) weigh2(s, c, r, j);
     }
     // A value that is not finite reaches the rows that see its key, and no others: the lane's channels (which are of one
     // block) become NaN in the rows that see a key of the tile whose block is NaN.
@@ -521,7 +528,9 @@ __device__ __attribute__((noinline)) void attn_mx8_f32(const __attribute__((addr
                     for (int r = 0; r < RG; r++)
                         s[r][h] = mx_mfma(mx_value((k[b >> 2] >> (8 * (b & 3))) & 255, x), gload<float>(w.query(r) + cc * 256 + 4 * b) * sign, s[r][h]);
             }
-        st.softmax(w, t, s, c);
+        float d[RG];
+        st.follow(w, t, s, c, d);
+        st.weigh(s, d);
         const bool whole = w.all_see(t, w.t_lo, w.t_hi);
         uint32_t x[8];
         bool bad = false;
@@ -551,7 +560,7 @@ template <int HD, int RG, bool TREE, bool WIDE>
 QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     using W = MxWork<HD, RG, TREE, WIDE>;
     using Tile = typename W::Tile;
-    constexpr int CC = W::CC, KS = W::KS, DT = W::DT, NB = W::NB, NCH = 2 * CC + DT / 2, MINE = NCH / 4;
+    constexpr int CC = W::CC, KS = W::KS, DT = W::DT, NB = W::NB;
     extern __shared__ float4 mx_lds[];
     const W w(a);
     if (w.b0 >= w.nrow) return;
@@ -613,74 +622,88 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     };
     MxState<HD, RG> st;
     st.start();
-    float cs[RG];          // score = accumulator times cs, in units of log2
-    int ek = -1, ev = -1;  // E of the keys and values, or -1: only zeros so far
+    int ek = 20, ev = 20;  // E of the keys and values (20 at least)
+    bool any_v = false;    // ev has been set
+    int moved = 0;         // the sums are to be multiplied by 2^moved (ev has changed)
+    float cs[RG];          // score = accumulator times cs, in units of log2, of keys unpacked with E = ek
+    auto unit = [&](int e, float (&c)[RG]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < RG; r++) cs[r] = 1.2e-38f;
+        for (int r = 0; r < RG; r++) c[r] = fmaxf(__builtin_ldexpf(scale, e + qe[r] - 152), 1.2e-38f);
+    };
     auto wave_most = [&](int x) __attribute__((always_inline)) {  // of whole numbers below 2^24
         return (int)__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max_v((float)x, lane))));
     };
-    // The tile's scales made ready: those of slots without a key (which may hold anything) 0, E such that all fit; false
-    // where no E will do.  Lanes that hold the same scales look at a part of them each: byte g of their keys' (hd = 64:
-    // g % 2), bytes n16 % 4 of their values'.
-    auto ready = [&](const Tile& t) __attribute__((always_inline)) {
-        if (!w.full(t)) {
+    // E for the scales lo .. hi of the lanes (lo: of those that are not 0, 65536 where all are), e for those before: e where
+    // it will do, else 4 above the largest or as far up as the smallest allows; 256 where no E will do.
+    auto settle = [&](int lo, int hi, int e) __attribute__((always_inline)) {
+        const int most = wave_most(hi), least = 65536 - wave_most(65536 - lo);
+        if (most == 0) return e;
+        if (most == (int)MX_NAN || least < most - 19) return 256;
+        return most > e || least < e - 19 ? max(min(min(most + 4, least + 19), 254), 20) : e;
+    };
+    // The scales of a tile's slots without a key (which may hold anything) become 0.
+    auto clear_k = [&](const Tile& t) __attribute__((always_inline)) {
+        if (w.full(t)) return;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                kx[h] = w.held(t, h * 16 + n16) ? kx[h] : 0;
+        for (int h = 0; h < 2; h++) kx[h] = w.held(t, h * 16 + n16) ? kx[h] : 0;
+    };
+    auto clear_v = [&](const Tile& t) __attribute__((always_inline)) {
+        if (w.full(t)) return;
 #pragma unroll
-                for (int j = 0; j < 4; j++) vx[h] &= w.held(t, h * 16 + 4 * g + j) ? 0xffffffffu : ~(255u << (8 * j));
-            }
-        }
-        const uint32_t ks = 8 * (g % NB), vs = 8 * (n16 & 3);
-        const int k0 = (kx[0] >> ks) & 255, k1 = (kx[1] >> ks) & 255;
-        int v0 = (vx[0] >> vs) & 255, v1 = (vx[1] >> vs) & 255;
-        const int kh = max(k0, k1);
-        int vh = max(v0, v1);
-        const int kl = min((k0 - 1) & 0xffff, (k1 - 1) & 0xffff) + 1;  // (0: no limit)
-        int vl = min((v0 - 1) & 0xffff, (v1 - 1) & 0xffff) + 1;
-        if (__all(kh <= ek && kl >= ek - 19 && vh <= ev && vl >= ev - 19)) return true;
-        // ---- seldom: the first tile, another E, blocks that are not finite
-        if (__any(vh == (int)MX_NAN) && !w.all_see(t, w.b_lo, w.b_hi)) {  // not every row sees every key: taken out
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) vx[h] &= w.held(t, h * 16 + 4 * g + j) ? 0xffffffffu : ~(255u << (8 * j));
+    };
+    // The least (of those that are not 0, 65536 where all are) and the largest scale that the lane looks at: lanes that hold the
+    // same ones look at a part of them each, byte g of their keys' (hd = 64: g % 2), bytes n16 % 4 of their values'.
+    struct Range { int lo, hi; };
+    auto range = [&](const uint32_t (&x)[2], uint32_t byte) __attribute__((always_inline)) {
+        const int a0 = (x[0] >> (8 * byte)) & 255, a1 = (x[1] >> (8 * byte)) & 255;
+        return Range{min((a0 - 1) & 0xffff, (a1 - 1) & 0xffff) + 1, max(a0, a1)};
+    };
+    auto range_k = [&]() __attribute__((always_inline)) { return range(kx, g % NB); };
+    auto range_v = [&]() __attribute__((always_inline)) { return range(vx, n16 & 3); };
+    auto fits = [&](Range x, int e) __attribute__((always_inline)) { return (x.hi <= e) & (x.lo >= e - 19); };
+    // E such that the tile's keys, its values fit; false where none will do.
+    auto settle_k = [&]() __attribute__((always_inline)) {
+        const Range x = range_k();
+        ek = settle(x.lo, x.hi, ek);
+        return ek < 256;
+    };
+    auto settle_v = [&](const Tile& t) __attribute__((always_inline)) {
+        Range x = range_v();
+        if (__any(x.hi == (int)MX_NAN) && !w.all_see(t, w.b_lo, w.b_hi)) {  // not every row sees every key: taken out
             st.poison(w, t);
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (((vx[i] >> (8 * j)) & 255) == MX_NAN) vx[i] &= ~(255u << (8 * j));
-            v0 = (vx[0] >> vs) & 255, v1 = (vx[1] >> vs) & 255;
-            vh = max(v0, v1);
-            vl = min((v0 - 1) & 0xffff, (v1 - 1) & 0xffff) + 1;
+            x = range_v();
         }
-        const int kmax = wave_most(kh), vmax = wave_most(vh), kmin = 65536 - wave_most(65536 - kl), vmin = 65536 - wave_most(65536 - vl);
-        if (max(kmax, vmax) == (int)MX_NAN || kmin < kmax - 19 || vmin < vmax - 19) return false;
-        if (kmax && (kmax > ek || kmin < ek - 19)) {
-            ek = min(min(kmax + 4, kmin + 19), 254);
+        const int e = settle(x.lo, x.hi, ev);
+        moved = any_v ? ev - e : 0;
+        any_v = any_v || __any(x.hi != 0);
+        ev = e;
+        return e < 256 && abs(moved) <= 60;  // (the sums could leave f32's range)
+    };
+    auto move = [&]() __attribute__((always_inline)) {
+        if (moved == 0) return;
 #pragma unroll
-            for (int r = 0; r < RG; r++) cs[r] = fmaxf(__builtin_ldexpf(scale, ek - 138 + qe[r] - 14), 1.2e-38f);
-        }
-        if (vmax && (vmax > ev || vmin < ev - 19)) {
-            const int e = min(min(vmax + 4, vmin + 19), 254);
-            if (ev >= 0) {
-                if (abs(e - ev) > 60) return false;  // (the sums could leave f32's range)
+        for (int r = 0; r < RG; r++)
 #pragma unroll
-                for (int r = 0; r < RG; r++)
+            for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int x = 0; x < 4; x++) st.o[r][d][x] = __builtin_ldexpf(st.o[r][d][x], ev - e);
-            }
-            ev = e;
-        }
-        return true;
+                for (int x = 0; x < 4; x++) st.o[r][d][x] = __builtin_ldexpf(st.o[r][d][x], moved);
+        moved = 0;
     };
     auto pair = [&](uint32_t v, uint32_t i, uint32_t j) __attribute__((always_inline)) {  // bytes i and j of v
         return __builtin_bit_cast(us2, __builtin_amdgcn_perm(0u, v, 0x0c000c00u | i | (j << 16)));
     };
     // 2^(x - E + 5) of two blocks as f16 (0 below the normal ones)
     auto factor = [&](us2 x, int e) __attribute__((always_inline)) {
-        const uint16_t lo = (uint16_t)max(e - 20, 0), up = (uint16_t)max(20 - max(e, 0), 0);  // (exponent 20: 2^5)
-        return __builtin_bit_cast(h2, (us2)((__builtin_elementwise_sub_sat(x, us2{lo, lo}) + us2{up, up}) << us2{10, 10}));
+        const uint16_t lo = (uint16_t)(e - 20);  // (exponent 20: 2^5)
+        return __builtin_bit_cast(h2, (us2)(__builtin_elementwise_sub_sat(x, us2{lo, lo}) << us2{10, 10}));
     };
     const h2 k1152 = {(_Float16)-1152.0f, (_Float16)-1152.0f};
     auto key_factors = [&](uint32_t x, int c, h2 (&s)[4], h2 (&off)[4]) __attribute__((always_inline)) {
@@ -690,13 +713,14 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
 #pragma unroll
         for (int i = 1; i < 4; i++) s[i] = s[0], off[i] = off[0];
     };
-    auto value_factors = [&](h2 (&s)[4], h2 (&off)[4]) __attribute__((always_inline)) {
+    auto value_factors = [&](const uint32_t (&x)[2], h2 (&s)[4], h2 (&off)[4]) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            s[c] = factor(pair(vx[c >> 1], 2 * (c & 1), 2 * (c & 1) + 1), ev);
+            s[c] = factor(pair(x[c >> 1], 2 * (c & 1), 2 * (c & 1) + 1), ev);
             off[c] = s[c] * k1152;
         }
     };
+    unit(ek, cs);
     // eight bytes q + 128 as f16 times the factors s (of two bytes each), off = -1152 s
     auto unpack8 = [&](uint32_t w0, uint32_t w1, const h2 (&s)[4], const h2 (&off)[4]) __attribute__((always_inline)) {
         h8 v;
@@ -709,27 +733,40 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
         return v;
     };
     h8 ph[RG], pl[RG];
-    auto split_p = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int r = 0; r < RG; r++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                ph[r][j] = (_Float16)(st.p[r][j] * MX_UP);
-                pl[r][j] = (_Float16)fmaf(st.p[r][j], MX_UP, -(float)ph[r][j]);
-            }
+    float one = 1.0f;  // (not known to the compiler: p - high in one instruction that takes an f16 operand)
+    asm("" : "+s"(one));
+    auto split2 = [&](int r, int j) __attribute__((always_inline)) {
+        // (rounded towards zero: the low part takes the rest, 21 bits together)
+        const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(st.p[r][j], st.p[r][j + 1]));
+        ph[r][j] = hi[0];
+        ph[r][j + 1] = hi[1];
+        pl[r][j] = (_Float16)fmaf(st.p[r][j], one, -(float)hi[0]);
+        pl[r][j + 1] = (_Float16)fmaf(st.p[r][j + 1], one, -(float)hi[1]);
     };
-    auto scores = [&](f32x4 (&s)[RG][2], int h, int c, h8 k) __attribute__((always_inline)) {
+    // Step c of the scores of both halves of the tile (their operands k0, k1), and the outputs d and d + 1 (v0, v1): no matrix
+    // instruction adds to the sums of the one before it, which it would wait for.
+    auto scores = [&](f32x4 (&s)[RG][2], int c, h8 k0, h8 k1) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < RG; r++) {
-            s[r][h] = mx_mfma(k, qh[r][c], c ? s[r][h] : f32x4{0, 0, 0, 0});
-            s[r][h] = mx_mfma(k, ql[r][c], s[r][h]);
+            s[r][0] = mx_mfma(k0, qh[r][c], c ? s[r][0] : f32x4{0, 0, 0, 0});
+            s[r][1] = mx_mfma(k1, qh[r][c], c ? s[r][1] : f32x4{0, 0, 0, 0});
+        }
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            s[r][0] = mx_mfma(k0, ql[r][c], s[r][0]);
+            s[r][1] = mx_mfma(k1, ql[r][c], s[r][1]);
         }
     };
-    auto outputs = [&](int d, h8 v) __attribute__((always_inline)) {
+    auto outputs = [&](int d, h8 v0, h8 v1) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < RG; r++) {
-            st.o[r][d] = mx_mfma(v, ph[r], st.o[r][d]);
-            st.o[r][d] = mx_mfma(v, pl[r], st.o[r][d]);
+            st.o[r][d] = mx_mfma(v0, ph[r], st.o[r][d]);
+            st.o[r][d + 1] = mx_mfma(v1, ph[r], st.o[r][d + 1]);
+        }
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            st.o[r][d] = mx_mfma(v0, pl[r], st.o[r][d]);
+            st.o[r][d + 1] = mx_mfma(v1, pl[r], st.o[r][d + 1]);
         }
     };
     bool ok = __syncthreads_and(alike) != 0;
@@ -753,83 +790,135 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
         load_v(i);
         for (; ok && i < i1; i += 4) {
             const Tile t = w.tile(i);
-            if (!ready(t)) {
-                ok = false;
-                break;
+            clear_k(t);
+            clear_v(t);
+            if (!__all(fits(range_k(), ek) & fits(range_v(), ev))) {
+                ok = settle_k() && settle_v(t);
+                if (!ok) break;
+                unit(ek, cs);
+                move();
             }
             f32x4 s[RG][2];
-            h2 f[4], off[4];
+            h2 f[4], off[4], f1[4], off1[4];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int c = 0; c < CC; c++) {
+                key_factors(kx[0], c, f, off);
+                key_factors(kx[1], c, f1, off1);
 #pragma unroll
-                for (int c = 0; c < CC; c++) {
-                    key_factors(kx[h], c, f, off);
-                    scores(s, h, 2 * c, unpack8(kw[h * CC + c][0], kw[h * CC + c][1], f, off));
-                    scores(s, h, 2 * c + 1, unpack8(kw[h * CC + c][2], kw[h * CC + c][3], f, off));
-                }
+                for (int u = 0; u < 2; u++)
+                    scores(s, 2 * c + u, unpack8(kw[c][2 * u], kw[c][2 * u + 1], f, off),
+                           unpack8(kw[CC + c][2 * u], kw[CC + c][2 * u + 1], f1, off1));
+            }
             load_k(i + 4);
-            st.softmax(w, t, s, cs);
-            split_p();
-            value_factors(f, off);
+            float c[RG];
+            st.follow(w, t, s, cs, c);
+            st.weigh(s, c);
 #pragma unroll
-            for (int d = 0; d < DT; d++) outputs(d, unpack8(vw[d >> 1][2 * (d & 1)], vw[d >> 1][2 * (d & 1) + 1], f, off));
+            for (int r = 0; r < RG; r++)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) split2(r, j);
+            value_factors(vx, f, off);
+#pragma unroll
+            for (int d = 0; d < DT; d += 2)
+                outputs(d, unpack8(vw[d >> 1][0], vw[d >> 1][1], f, off), unpack8(vw[d >> 1][2], vw[d >> 1][3], f, off));
             load_v(i + 4);
         }
         ok = __syncthreads_and(ok) != 0;
     } else {
-        // every wavefront takes every tile, of which each unpacks a quarter to f16 in LDS (two buffers): chunk c of a tile
-        // (1 KB: of K below 2 CC, then of V) is the wavefront's where c % 4 == wave
+        // Every wavefront takes every tile, of which each unpacks a chunk of 1 KB to f16 in LDS (two buffers): chunk c (of K
+        // below 2 CC, then of V) is wavefront c's.  It looks at that chunk's scales alone; where they do not fit E, it leaves a
+        // word in LDS (one for each buffer), and all settle E anew and unpack the tile again.
+        constexpr uint32_t NCH = 2 * CC + DT / 2;
         h8* lds = reinterpret_cast<h8*>(mx_lds);  // [buffer][chunk][half of the lane's bytes][lane]
-        u32x4 raw[MINE];
-        auto load = [&](uint32_t j) __attribute__((always_inline)) {
-            const uint32_t at = j < i1 ? w.tile(j).slot * HD + lane * 16 : QP_NOOFF;
-            load_kx(j);
-            load_vx(j);
-#pragma unroll
-            for (int u = 0; u < MINE; u++) {
-                const uint32_t c = wave + 4 * u;
-                raw[u] = c < 2 * CC ? __builtin_amdgcn_raw_buffer_load_b128(kr, at, c * 1024, 0)
-                                    : __builtin_amdgcn_raw_buffer_load_b128(vr, at, (c - 2 * CC) * 1024, 0);
+        volatile uint32_t* misfit = reinterpret_cast<volatile uint32_t*>(lds + 2 * NCH * 128);
+        const bool is_k = wave < 2 * CC, has = wave < NCH;
+        const __amdgpu_buffer_rsrc_t mine = is_k ? kr : vr, mine_x = is_k ? kxr : vxr;
+        const uint32_t at = (is_k ? wave : wave - 2 * CC) * 1024 + lane * 16;
+        const uint32_t at_x = is_k ? ((wave / CC) * 16 + n16) * NB : (n16 * DT / 32) * 32 + g * 8;
+        u32x4 raw;
+        uint32_t x[2];  // the chunk's scales: K's of the lane's key, V's of its 8 keys
+        auto load = [&](uint32_t j) __attribute__((always_inline)) {  // (past the last tile: the last)
+            const uint32_t slot = w.tile(min(j, i1 - 1)).slot;
+            if (is_k && NB == 2) {
+                x[0] = __builtin_amdgcn_raw_buffer_load_b16(mine_x, at_x, slot * NB, 0);
+            } else if (is_k) {
+                x[0] = __builtin_amdgcn_raw_buffer_load_b32(mine_x, at_x, slot * NB, 0);
+            } else if (has) {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b64(mine_x, at_x, slot * NB, 0);
+                x[0] = v[0];
+                x[1] = v[1];
             }
+            if (has) raw = __builtin_amdgcn_raw_buffer_load_b128(mine, at, slot * HD, 0);
         };
         auto stage = [&](uint32_t j) __attribute__((always_inline)) {
+            if (!has) return;
+            const Tile t = w.tile(j);
+            h2 f[4], off[4];
+            bool fit;
+            if (is_k) {
+                if (!w.full(t)) x[0] = w.held(t, (wave / CC) * 16 + n16) ? x[0] : 0;
+                const int b = (x[0] >> (8 * (2 * (wave % CC) + (g >> 1)))) & 255;
+                fit = (b <= ek) & ((b >= ek - 19) | (b == 0));
+                key_factors(x[0], wave % CC, f, off);
+            } else {
+                if (!w.full(t)) {
 #pragma unroll
-            for (int u = 0; u < MINE; u++) {
-                const uint32_t c = wave + 4 * u;
-                h2 f[4], off[4];
-                if (c < 2 * CC) key_factors(c / CC ? kx[1] : kx[0], c % CC, f, off);
-                else value_factors(f, off);
-                h8* to = lds + ((j & 1) * NCH + c) * 128 + lane;
-                to[0] = unpack8(raw[u][0], raw[u][1], f, off);
-                to[64] = unpack8(raw[u][2], raw[u][3], f, off);
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) x[h] &= w.held(t, h * 16 + 4 * g + j) ? 0xffffffffu : ~(255u << (8 * j));
+                }
+                fit = fits(range(x, n16 & 3), ev);
+                value_factors(x, f, off);
             }
+            if (!__all(fit) && lane == 0) misfit[j & 1] = 1;
+            h8* to = lds + ((j & 1) * NCH + wave) * 128 + lane;
+            to[0] = unpack8(raw[0], raw[1], f, off);
+            to[64] = unpack8(raw[2], raw[3], f, off);
         };
         uint32_t i = w.i0;
         if (ok && i < i1) {
-            load(i);
-            ok = ready(w.tile(i));
-            if (ok) stage(i);
-            load(i + 1);
-            __syncthreads();
-            while (ok) {
+            bool settle_now = true;  // (the first tile)
+            if (threadIdx.x < 2) misfit[threadIdx.x] = 0;
+            for (;;) {
                 const Tile t = w.tile(i);
+                if (settle_now) {
+                    __syncthreads();
+                    load(i);
+                    load_kx(i);
+                    load_vx(i);
+                    clear_k(t);
+                    clear_v(t);
+                    ok = settle_k() && settle_v(t);  // (the same in all wavefronts: they see the same scales)
+                    if (!ok) break;
+                    unit(ek, cs);
+                    move();
+                    // (blocks that settle_v took out: unpacked as 0)
+                    if (!is_k) x[0] = vx[0], x[1] = vx[1];
+                    if (threadIdx.x == 0) misfit[i & 1] = 0;
+                    stage(i);
+                    load(i + 1);
+                    __syncthreads();
+                }
                 if (w.wanted(t)) {
                     const h8* from = lds + (i & 1) * NCH * 128 + lane;
                     f32x4 s[RG][2];
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int c = 0; c < KS; c++) scores(s, c, from[c * 64], from[(KS + c) * 64]);
+                    float c[RG];
+                    st.follow(w, t, s, cs, c);
+                    st.weigh(s, c);
 #pragma unroll
-                        for (int c = 0; c < KS; c++) scores(s, h, c, from[(h * KS + c) * 64]);
-                    st.softmax(w, t, s, cs);
-                    split_p();
+                    for (int r = 0; r < RG; r++)
 #pragma unroll
-                    for (int d = 0; d < DT; d++) outputs(d, from[(2 * KS + d) * 64]);
+                        for (int j = 0; j < 8; j += 2) split2(r, j);
+#pragma unroll
+                    for (int d = 0; d < DT; d += 2) outputs(d, from[(2 * KS + d) * 64], from[(2 * KS + d + 1) * 64]);
                 }
                 if (++i >= i1) break;
-                ok = ready(w.tile(i));  // (the same in all wavefronts: they see the same scales)
-                if (ok) stage(i);
+                stage(i);
                 load(i + 1);
                 __syncthreads();
+                settle_now = __builtin_amdgcn_readfirstlane(misfit[i & 1]) != 0;
             }
         }
     }
@@ -837,7 +926,7 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
         attn_mx8_f32<HD, RG, TREE, WIDE>((const __attribute__((address_space(4))) QpAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr());
         return;
     }
-    const int back = max(ev, 0) - 138 - 12;  // o times 2^back: the outputs
+    const int back = ev - 138;  // o times 2^back: the outputs
     st.sum_l(lane);
     if constexpr (WIDE) {
         st.put_all(w, back);
@@ -888,8 +977,8 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
         QpAttnArgs a) { attn_mx8_body<HD, 1, TREE, false>(a); }                                                       \
     KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void qp_attn_mx8_h##HD##_##NAME##_r2(       \
         QpAttnArgs a) { attn_mx8_body<HD, 2, TREE, false>(a); }                                                       \
-    KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void qp_attn_mx8_h##HD##_##NAME##_wide(     \
-        QpAttnArgs a) { attn_mx8_body<HD, 2, TREE, true>(a); }
+    KERNEL __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void qp_attn_mx8_h##HD##_##NAME##_wide(     \
+        QpAttnArgs a) { attn_mx8_body<HD, 1, TREE, true>(a); }
 ATTN_MX8(64, causal, false) ATTN_MX8(128, causal, false) ATTN_MX8(64, tree, true) ATTN_MX8(128, tree, true)
 
 // The shares' partial states of each (query, head) row -> o, in their order: grid rows, hd threads (at most 64 shares).

@@ -1201,8 +1201,8 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
                                     {{K_attn_t_h64_f16_r1, K_attn_t_h64_f16_r2}, {K_attn_t_h128_f16_r1, K_attn_t_h128_f16_r2}}};
     static const Kid kw[2][2] = {{K_attn_mx8_h64_causal_wide, K_attn_mx8_h128_causal_wide}, {K_attn_mx8_h64_tree_wide, K_attn_mx8_h128_tree_wide}};
     const Kid k = wide ? kw[tree][a.hd == 128] : fmt == QP_KV_MX8 ? k8[tree][a.hd == 128][RG == 2] : kt[fmt][a.hd == 128][RG == 2];
-    const uint32_t lds = wide ? 2 * 128 * a.hd : 4 * RG * 16 * (a.hd + 4) * 4 + 4 * RG * 16 * 8;
-    if (int e = launch(k, a.nkv, yb, ns, 256, lds, a)) return e;
+    const uint32_t lds = wide ? 2 * 128 * a.hd + 16 : 4 * RG * 16 * (a.hd + 4) * 4 + 4 * RG * 16 * 8;
+    if (int e = launch(k, a.nkv, yb, ns, wide ? 512 : 256, lds, a)) return e;
     return ns == 1 ? 0 : launch(K_attn_mx8_comb, T * a.nh, 1, 1, a.hd, 0, a);
 }
 
