@@ -288,13 +288,17 @@ struct MxWork {
     QP_DEV MxWork(const QpAttnArgs& args) : a(args) {
         lane = threadIdx.x & 63, g = lane >> 4, n16 = lane & 15;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        T = min(__builtin_amdgcn_readfirstlane(paso_T(a.paso)), a.tcov), pos0 = __builtin_amdgcn_readfirstlane(paso_pos(a.paso));
-        G = a.nh / a.nkv, kvh = blockIdx.x, nrow = T * G, R = mx_slots(a.rows);
+        G = a.nh / a.nkv, kvh = blockIdx.x, R = mx_slots(a.rows);
         // long prompts: the blocks with the most keys first, then those with the fewest on (two workgroups share a CU)
         const uint32_t y = blockIdx.y, ny = gridDim.y, blk = TREE ? y : y < (ny + 1) / 2 ? ny - 1 - y : y - (ny + 1) / 2;
         b0 = blk * (WIDE ? 128 * RG : 16 * RG);
         r0 = b0 + (WIDE ? wave * 16 * RG : 0);
-        if (b0 >= nrow) return;
+    }
+    // What depends on the Paso; false where it has no rows for the workgroup.
+    QP_DEV bool begin() {
+        const uint2 paso = gload<uint2>(a.paso);
+        T = min(__builtin_amdgcn_readfirstlane(paso.x), a.tcov), pos0 = __builtin_amdgcn_readfirstlane(paso.y), nrow = T * G;
+        if (b0 >= nrow) return false;
         b_lo = b0 / G, b_hi = (min(b0 + (WIDE ? 128 * RG : 16 * RG), nrow) - 1) / G;
         t_lo = min(r0, nrow - 1) / G, t_hi = (min(r0 + 16 * RG, nrow) - 1) / G;
 #pragma unroll
@@ -318,9 +322,10 @@ struct MxWork {
         const uint32_t nt = ta + (end_b + 31) / 32, per = (nt + a.nsplit - 1) / a.nsplit;
         i0 = blockIdx.z * per, i1 = min(nt, i0 + per);
         hk = (uint64_t)kvh * R * HD, hx = (uint64_t)a.nkv * R * HD + (uint64_t)kvh * R * NB;
+        return true;
     }
-    // the lane's row of group r (past the last: the last), and its query from the lane's inputs on
-    QP_DEV uint32_t row(int r) const { return min(r0 + r * 16 + n16, nrow - 1); }
+    // the lane's row of group r (past those that the dispatch covers: the last), and its query from the lane's inputs on
+    QP_DEV uint32_t row(int r) const { return min(r0 + r * 16 + n16, a.tcov * G - 1); }
     QP_DEV uint64_t query(int r) const {
         const uint32_t rc = row(r);
         return a.q + 4 * (((uint64_t)(rc / G) * a.nh + kvh * G + rc % G) * HD + 16 * g);
@@ -501,8 +506,8 @@ template <int HD, int RG, bool TREE, bool WIDE>
 __device__ __attribute__((noinline)) void attn_mx8_f32(const __attribute__((address_space(4))) QpAttnArgs* args) {
     const QpAttnArgs a = *args;
     using W = MxWork<HD, RG, TREE, WIDE>;
-    const W w(a);
-    if (WIDE ? w.r0 >= w.nrow : w.wave != 0) return;
+    W w(a);
+    if (!w.begin() || (WIDE ? w.r0 >= w.nrow : w.wave != 0)) return;
     MxState<HD, RG> st;
     st.start();
     const float scale = a.scale * MX_LOG2E, sign = scale < 0.0f ? -1.0f : 1.0f;
@@ -562,21 +567,64 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     using Tile = typename W::Tile;
     constexpr int CC = W::CC, KS = W::KS, DT = W::DT, NB = W::NB;
     extern __shared__ float4 mx_lds[];
-    const W w(a);
-    if (w.b0 >= w.nrow) return;
-    const uint32_t lane = w.lane, g = w.g, n16 = w.n16, wave = w.wave;
+    W w(a);
+    // The queries' loads do not wait for the Paso, the first tiles' not for the queries (one token behind 4100 keys: 9.4 us,
+    // 10.0 with each after the other).
+    float4 qv[RG][KS][2];
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+        const uint64_t at = w.query(r);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) qv[r][s][i] = gload<float4>(at + (s >> 1) * 256 + (s & 1) * 32 + i * 16);
+    }
+    if (!w.begin()) return;
+    const uint32_t lane = w.lane, g = w.g, n16 = w.n16, wave = w.wave, i1 = w.i1;
     const float scale = fabsf(a.scale) * MX_LOG2E;
+    const __amdgpu_buffer_rsrc_t kr = kq_rsrc(a.kc + w.hk, (uint64_t)w.R * HD), vr = kq_rsrc(a.vc + w.hk, (uint64_t)w.R * HD);
+    const __amdgpu_buffer_rsrc_t kxr = kq_rsrc(a.kc + w.hx, (uint64_t)w.R * NB), vxr = kq_rsrc(a.vc + w.hx, (uint64_t)w.R * NB);
+    uint32_t kx[2], vx[2];  // the scales of the lane's key of each half, and of its 8 values' keys
+    auto load_kx = [&](uint32_t i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t x = i < i1 ? (w.tile(i).slot + h * 16 + n16) * NB : QP_NOOFF;
+            if constexpr (NB == 4) kx[h] = __builtin_amdgcn_raw_buffer_load_b32(kxr, x, 0, 0);
+            else kx[h] = __builtin_amdgcn_raw_buffer_load_b16(kxr, x, 0, 0);
+        }
+    };
+    auto load_vx = [&](uint32_t i) __attribute__((always_inline)) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b64(vxr, i < i1 ? w.tile(i).slot * NB + (n16 * DT / 32) * 32 + g * 8 : QP_NOOFF, 0, 0);
+        vx[0] = x[0];
+        vx[1] = x[1];
+    };
+    u32x4 kw[2 * CC], vw[DT / 2];  // not WIDE: the wavefront's tile
+    auto load_k = [&](uint32_t i) __attribute__((always_inline)) {
+        const uint32_t o = i < i1 ? w.tile(i).slot * HD + lane * 16 : QP_NOOFF;
+        load_kx(i);
+#pragma unroll
+        for (int c = 0; c < 2 * CC; c++) kw[c] = __builtin_amdgcn_raw_buffer_load_b128(kr, o, c * 1024, 0);
+    };
+    auto load_v = [&](uint32_t i) __attribute__((always_inline)) {
+        const uint32_t o = i < i1 ? w.tile(i).slot * HD + lane * 16 : QP_NOOFF;
+        load_vx(i);
+#pragma unroll
+        for (int c = 0; c < DT / 2; c++) vw[c] = __builtin_amdgcn_raw_buffer_load_b128(vr, o, c * 1024, 0);
+    };
+    if constexpr (!WIDE) {
+        load_k(w.i0 + wave);
+        load_v(w.i0 + wave);
+    }
     // ---- the rows' queries
     h8 qh[RG][KS], ql[RG][KS];
     int qe[RG];
     bool alike = true;  // the lane's fit the f16 parts
 #pragma unroll
     for (int r = 0; r < RG; r++) {
-        const uint64_t at = w.query(r);
         float v[KS][8], mine = 0.0f, least = 3.4e38f;  // the largest element, the least of the largest of 8 (not 0)
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            const float4 x = gload<float4>(at + (s >> 1) * 256 + (s & 1) * 32), z = gload<float4>(at + (s >> 1) * 256 + (s & 1) * 32 + 16);
+            const float4 x = qv[r][s][0], z = qv[r][s][1];
             const float f[8] = {x.x, x.y, x.z, x.w, z.x, z.y, z.z, z.w};
             float eight = 0.0f;
 #pragma unroll
@@ -603,23 +651,6 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
                 ql[r][s][i] = (_Float16)(x - (float)qh[r][s][i]);
             }
     }
-    const uint32_t i1 = w.i1;
-    const __amdgpu_buffer_rsrc_t kr = kq_rsrc(a.kc + w.hk, (uint64_t)w.R * HD), vr = kq_rsrc(a.vc + w.hk, (uint64_t)w.R * HD);
-    const __amdgpu_buffer_rsrc_t kxr = kq_rsrc(a.kc + w.hx, (uint64_t)w.R * NB), vxr = kq_rsrc(a.vc + w.hx, (uint64_t)w.R * NB);
-    uint32_t kx[2], vx[2];  // the scales of the lane's key of each half, and of its 8 values' keys
-    auto load_kx = [&](uint32_t i) __attribute__((always_inline)) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const uint32_t x = i < i1 ? (w.tile(i).slot + h * 16 + n16) * NB : QP_NOOFF;
-            if constexpr (NB == 4) kx[h] = __builtin_amdgcn_raw_buffer_load_b32(kxr, x, 0, 0);
-            else kx[h] = __builtin_amdgcn_raw_buffer_load_b16(kxr, x, 0, 0);
-        }
-    };
-    auto load_vx = [&](uint32_t i) __attribute__((always_inline)) {
-        const auto x = __builtin_amdgcn_raw_buffer_load_b64(vxr, i < i1 ? w.tile(i).slot * NB + (n16 * DT / 32) * 32 + g * 8 : QP_NOOFF, 0, 0);
-        vx[0] = x[0];
-        vx[1] = x[1];
-    };
     MxState<HD, RG> st;
     st.start();
     int ek = 20, ev = 20;  // E of the keys and values (20 at least)
@@ -772,22 +803,7 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     bool ok = __syncthreads_and(alike) != 0;
     if constexpr (!WIDE) {
         // the tiles are dealt to the wavefronts, each with a state of its own
-        u32x4 kw[2 * CC], vw[DT / 2];
-        auto load_k = [&](uint32_t i) __attribute__((always_inline)) {
-            const uint32_t o = i < i1 ? w.tile(i).slot * HD + lane * 16 : QP_NOOFF;
-            load_kx(i);
-#pragma unroll
-            for (int c = 0; c < 2 * CC; c++) kw[c] = __builtin_amdgcn_raw_buffer_load_b128(kr, o, c * 1024, 0);
-        };
-        auto load_v = [&](uint32_t i) __attribute__((always_inline)) {
-            const uint32_t o = i < i1 ? w.tile(i).slot * HD + lane * 16 : QP_NOOFF;
-            load_vx(i);
-#pragma unroll
-            for (int c = 0; c < DT / 2; c++) vw[c] = __builtin_amdgcn_raw_buffer_load_b128(vr, o, c * 1024, 0);
-        };
         uint32_t i = w.i0 + wave;
-        load_k(i);
-        load_v(i);
         for (; ok && i < i1; i += 4) {
             const Tile t = w.tile(i);
             clear_k(t);
@@ -973,10 +989,8 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
 }
 
 #define ATTN_MX8(HD, NAME, TREE)                                                                                      \
-    KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void qp_attn_mx8_h##HD##_##NAME##_r1(       \
+    KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void qp_attn_mx8_h##HD##_##NAME(            \
         QpAttnArgs a) { attn_mx8_body<HD, 1, TREE, false>(a); }                                                       \
-    KERNEL __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void qp_attn_mx8_h##HD##_##NAME##_r2(       \
-        QpAttnArgs a) { attn_mx8_body<HD, 2, TREE, false>(a); }                                                       \
     KERNEL __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void qp_attn_mx8_h##HD##_##NAME##_wide(     \
         QpAttnArgs a) { attn_mx8_body<HD, 1, TREE, true>(a); }
 ATTN_MX8(64, causal, false) ATTN_MX8(128, causal, false) ATTN_MX8(64, tree, true) ATTN_MX8(128, tree, true)
@@ -985,17 +999,17 @@ ATTN_MX8(64, causal, false) ATTN_MX8(128, causal, false) ATTN_MX8(64, tree, true
 // A row that no share saw a key of is 0.
 KERNEL __launch_bounds__(128) void qp_attn_mx8_comb(QpAttnArgs a) {
     __shared__ float wt[64], den;
-    const uint32_t t = blockIdx.x / a.nh, d = threadIdx.x, ns = a.nsplit;
-    if (t >= paso_T(a.paso)) return;
+    const uint32_t t = blockIdx.x / a.nh, d = threadIdx.x, ns = a.nsplit, T = paso_T(a.paso);
     const uint64_t row = blockIdx.x, po = a.part_o + 4 * (row * ns * a.hd + d);
     float v[8];
 #pragma unroll
     for (uint32_t s = 0; s < 8; s++) v[s] = s < ns ? gload<float>(po + 4ull * s * a.hd) : 0.0f;
+    const float2 mine = d < ns ? gload<float2>(a.part_ml + 8 * (row * ns + d)) : make_float2(-3.0e38f, 0.0f);
+    if (t >= T) return;  // (the loads above are of the buffer all the same)
     if (d < 64) {
-        const float2 ml = d < ns ? gload<float2>(a.part_ml + 8 * (row * ns + d)) : make_float2(-3.0e38f, 0.0f);
-        const float M = wave_max_v(ml.x, d), f = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - M) : -1.0f;
+        const float M = wave_max_v(mine.x, d), f = mine.y != 0.0f ? __builtin_amdgcn_exp2f(mine.x - M) : -1.0f;
         wt[d] = f;
-        const float L = wave_sum_v(ml.y != 0.0f ? ml.y * f : 0.0f, d);
+        const float L = wave_sum_v(mine.y != 0.0f ? mine.y * f : 0.0f, d);
         if (d == 0) den = L;
     }
     __syncthreads();

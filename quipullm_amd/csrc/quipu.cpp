@@ -1164,13 +1164,16 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     const uint64_t qb = 4ull * T * a.nh * a.hd;
     if (int e = need_room(a.q, qb, op, "q")) return e;
     if (int e = need_room(a.o, qb, op, "the output")) return e;
-    const uint64_t nrow = (uint64_t)T * G;
-#ifndef MX_WIDE_FROM
-#define MX_WIDE_FROM 65
-#endif
-    const bool wide = fmt == QP_KV_MX8 && nrow >= MX_WIDE_FROM;
-    const uint32_t RG = nrow > 16 ? 2 : 1, block = wide ? 128 : 16 * RG;
-    if (cdiv(nrow, block) > 65535) return fail(QP_E_ARG, "%s: %u tokens in one call", op, T);
+    const uint32_t cus = g_cus > 0 ? (uint32_t)g_cus : 1u;
+    const uint64_t nrow = (uint64_t)T * G, keys = a.swa && (uint64_t)a.swa + T < a.rows ? a.swa + T : a.rows;
+    // 8-bit caches: blocks of 128 rows, whose wavefronts share the unpacked tiles, where there are enough of them for the
+    // device's CUs, two on each where every share of the keys has 512 (8B shape, 2048 tokens: 108 us, 156 with blocks of 16
+    // rows; 512 behind 8000: 158 and 213; a tree of 64 behind 32700: 90 and 115); else blocks of 16 rows (512 tokens without a
+    // past: 26 us, 38 with 128; 32 behind 480: 15 and 20).  f32 and f16 caches: 16 or 32 rows.
+    const uint64_t yw = (nrow + 127) / 128;
+    const bool mx8 = fmt == QP_KV_MX8, wide = mx8 && nrow > 64 && (a.nkv * yw >= cus || a.nkv * yw * cdiv(keys, 512) >= 2 * cus);
+    const uint32_t RG = !mx8 && nrow > 16 ? 2 : 1, block = wide ? 128 : 16 * RG;
+    if ((nrow + block - 1) / block > 65535) return fail(QP_E_ARG, "%s: %u tokens in one call", op, T);
     const uint32_t yb = cdiv(nrow, block);
     const uint64_t per = (uint64_t)T * a.nh * (4 * a.hd + 8);  // bytes of one share's partial states
     if (ns > 64) return fail(QP_E_ARG, "%s: %u shares of the keys (at most 64)", op, ns);
@@ -1179,10 +1182,11 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
         if (int e = need_room(parts, ns * per, op, "the shares' buffer")) return e;
         a.part_o = parts;
     } else if (!ns) {
-        const uint32_t cus = g_cus > 0 ? (uint32_t)g_cus : 1u;
-        const uint64_t keys = a.swa && (uint64_t)a.swa + T < a.rows ? a.swa + T : a.rows;
-        ns = cdiv(cus, a.nkv * yb);
-        if (ns > cdiv(keys, 128)) ns = cdiv(keys, 128);
+        // shares of 256 keys or more (512 in blocks of 128 rows), while they make at most two workgroups for each CU; none
+        // where the blocks alone are one for each (one token behind 4100 keys in 18 shares: 13.4 us, in 32 14.0)
+        const uint32_t wgs = a.nkv * yb;
+        ns = wgs >= cus ? 1 : cdiv(2 * cus, wgs);
+        if (ns > cdiv(keys, wide ? 512 : 256)) ns = cdiv(keys, wide ? 512 : 256);
         if (ns > 64) ns = 64;
         if (g_capturing && !g_noalloc) ns = 1;
         if (g_noalloc && ns * per > QP_SCRATCH_BYTES) ns = 1;
@@ -1195,12 +1199,11 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     a.tcov = T;
     a.nsplit = ns;
     a.part_ml = ns > 1 ? a.part_o + 4ull * T * a.nh * ns * a.hd : 0;
-    static const Kid k8[2][2][2] = {{{K_attn_mx8_h64_causal_r1, K_attn_mx8_h64_causal_r2}, {K_attn_mx8_h128_causal_r1, K_attn_mx8_h128_causal_r2}},
-                                    {{K_attn_mx8_h64_tree_r1, K_attn_mx8_h64_tree_r2}, {K_attn_mx8_h128_tree_r1, K_attn_mx8_h128_tree_r2}}};
+    static const Kid k8[2][2][2] = {{{K_attn_mx8_h64_causal, K_attn_mx8_h64_causal_wide}, {K_attn_mx8_h128_causal, K_attn_mx8_h128_causal_wide}},
+                                    {{K_attn_mx8_h64_tree, K_attn_mx8_h64_tree_wide}, {K_attn_mx8_h128_tree, K_attn_mx8_h128_tree_wide}}};
     static const Kid kt[2][2][2] = {{{K_attn_t_h64_f32_r1, K_attn_t_h64_f32_r2}, {K_attn_t_h128_f32_r1, K_attn_t_h128_f32_r2}},
                                     {{K_attn_t_h64_f16_r1, K_attn_t_h64_f16_r2}, {K_attn_t_h128_f16_r1, K_attn_t_h128_f16_r2}}};
-    static const Kid kw[2][2] = {{K_attn_mx8_h64_causal_wide, K_attn_mx8_h128_causal_wide}, {K_attn_mx8_h64_tree_wide, K_attn_mx8_h128_tree_wide}};
-    const Kid k = wide ? kw[tree][a.hd == 128] : fmt == QP_KV_MX8 ? k8[tree][a.hd == 128][RG == 2] : kt[fmt][a.hd == 128][RG == 2];
+    const Kid k = mx8 ? k8[tree][a.hd == 128][wide] : kt[fmt][a.hd == 128][RG == 2];
     const uint32_t lds = wide ? 2 * 128 * a.hd + 16 : 4 * RG * 16 * (a.hd + 4) * 4 + 4 * RG * 16 * 8;
     if (int e = launch(k, a.nkv, yb, ns, wide ? 512 : 256, lds, a)) return e;
     return ns == 1 ? 0 : launch(K_attn_mx8_comb, T * a.nh, 1, 1, a.hd, 0, a);
