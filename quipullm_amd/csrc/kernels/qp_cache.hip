@@ -68,89 +68,138 @@ QP_DEV void sincos_far(float x, float& sn_out, float& cs_out) {
     cs_out = q == 1 || q == 2 ? -b : b;
 }
 
-// One wavefront (hd = 128) or half of one (hd = 64) per token and head of q, k or v; grid (T, ceil((nh + 2 nkv) / heads per
-// workgroup)).  A lane takes the two elements of a pair, norms and rotates them, then (through LDS where pairs are not
-// neighbours) two neighbouring channels, which it stores.
-KERNEL __launch_bounds__(256) void qp_norm_rope_kv(QpRopeKvArgs a) {
-    __shared__ float row_s[4][128];
-    const uint32_t t = blockIdx.x, hl = a.hd >> 1;             // lanes per head
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (hl - 1);
-    const uint32_t per = 256 / hl, head = blockIdx.y * per + threadIdx.x / hl;
-    if (t >= paso_T(a.paso)) return;
-    const uint32_t nq = a.nh, nall = a.nh + 2 * a.nkv;
-    const bool on = head < nall, isq = head < nq, isv = head >= nq + a.nkv;
-    const uint32_t h = isq ? head : isv ? head - nq - a.nkv : head - nq;
-    const uint64_t src = (isq ? a.q : isv ? a.v : a.k) + 4ull * (((uint64_t)t * (isq ? a.nh : a.nkv) + h) * a.hd);
-    const uint32_t half = a.nrot >> 1;
-    const bool apart = a.neox && !isv;                          // pairs (j, j + nrot / 2)
-    const uint32_t i0 = apart && l < half ? l : 2 * l, i1 = apart && l < half ? l + half : 2 * l + 1;
-    float x0 = on ? gload<float>(src + 4 * i0) : 0.0f, x1 = on ? gload<float>(src + 4 * i1) : 0.0f;
+// 1 / sqrt(y) for y >= 0 (off by one step at most; the instruction takes no subnormal y)
+QP_DEV float rsqrt_any(float y) {
+    const bool tiny = y < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? y * 0x1p100f : y);
+    return tiny ? r * 0x1p50f : r;
+}
+
+// A wavefront has one token (hd = 128) or two (hd = 64) of N heads of q, of k or of v, which share the token's angles; grid
+// (ceil(T / tokens), ceil(groups of N heads / 4)).  A lane takes the two elements of a pair, norms and rotates them, then
+// (through LDS where pairs are not neighbours) two neighbouring channels, which it stores.  With a token's 48 heads one by one
+// it is bound by the latency of its loads (T = 1, 8B shape: 2.7 us); with many tokens it was by the instructions for each head
+// (2048 tokens of 32 + 2 x 4 heads of 128: 30.4 us), hence the kind of head and the addresses in scalar registers and the angles
+// once for four heads: 17.7 us, 4.2 TB/s.
+template <int HD, int N>
+QP_DEV void norm_rope_kv_body(const QpRopeKvArgs& a) {
+    __shared__ float row_s[4][N][128];
+    constexpr uint32_t HL = HD / 2, TW = 128 / HD;              // lanes per head, tokens of a wavefront
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & (HL - 1);
+    const uint32_t nq = a.nh, gq = (nq + N - 1) / N, gk = (a.nkv + N - 1) / N, group = blockIdx.y * 4 + wave;
+    if (group >= gq + 2 * gk) return;
+    const bool isq = group < gq, isv = group >= gq + gk;
+    const uint32_t h0 = (isq ? group : isv ? group - gq - gk : group - gq) * N, nx = isq ? nq : a.nkv;
+    const uint32_t t0 = blockIdx.x * TW, t = t0 + lane / HL, half = isv ? 0 : a.nrot >> 1;
+    const bool apart = a.neox && l < half;                      // pairs (j, j + nrot / 2)
+    const uint32_t i0 = apart ? l : 2 * l, i1 = apart ? l + half : 2 * l + 1, row0 = lane / HL * nx * HD;
+    const uint64_t in = (isq ? a.q : isv ? a.v : a.k) + 4 * ((uint64_t)t0 * nx + h0) * HD;
+    const bool covered = t < a.tcov;
+    float x0[N], x1[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) {  // (the loads are of the call's T rows, whatever the Paso says)
+        const bool on = covered && h0 + n < nx;
+        x0[n] = on ? gload<float>(in + n * HD * 4 + (row0 + i0) * 4) : 0.0f;
+        x1[n] = on ? gload<float>(in + n * HD * 4 + (row0 + i1) * 4) : 0.0f;
+    }
     const uint64_t w = isv ? 0 : isq ? a.qnorm : a.knorm;
-    float ss = x0 * x0 + x1 * x1;
-    ss += bfly_f<0>(ss, lane);
-    ss += bfly_f<1>(ss, lane);
-    ss += bfly_f<2>(ss, lane);
-    ss += bfly_f<3>(ss, lane);
-    ss += bfly_f<4>(ss, lane);
-    if (hl == 64) ss += bfly_f<5>(ss, lane);
+    const float w0 = w ? gload<float>(w + 4 * i0) : 1.0f, w1 = w ? gload<float>(w + 4 * i1) : 1.0f;
+    const float freq = l < half ? gload<float>(a.freq + 4 * l) : 0.0f;
+    const uint2 paso = gload<uint2>(a.paso);
+    const uint32_t T = min(__builtin_amdgcn_readfirstlane(paso.x), a.tcov), pos0 = __builtin_amdgcn_readfirstlane(paso.y);
+    const uint32_t pos = a.pos && covered ? cptr<uint32_t>(a.pos)[t] : pos0 + t;
+    if (t0 >= T) return;
     if (w) {
-        const float inv = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
-        x0 = (x0 * inv) * gload<float>(w + 4 * i0);
-        x1 = (x1 * inv) * gload<float>(w + 4 * i1);
+        float ss[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) ss[n] = x0[n] * x0[n] + x1[n] * x1[n];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            ss[n] += bfly_f<0>(ss[n], lane);
+            ss[n] += bfly_f<1>(ss[n], lane);
+            ss[n] += bfly_f<2>(ss[n], lane);
+            ss[n] += bfly_f<3>(ss[n], lane);
+            ss[n] += bfly_f<4>(ss[n], lane);
+            if constexpr (HL == 64) ss[n] += bfly_f<5>(ss[n], lane);
+            const float inv = rsqrt_any(ss[n] * (1.0f / HD) + a.eps);
+            x0[n] = (x0[n] * inv) * w0;
+            x1[n] = (x1[n] * inv) * w1;
+        }
     }
-    if (!isv && l < half) {
-        const uint32_t pos = a.pos ? cptr<uint32_t>(a.pos)[t] : paso_pos(a.paso) + t;
+    if (half) {
         float sn, cs;
-        sincos_far(((float)pos * a.esc) * gload<float>(a.freq + 4 * l), sn, cs);
-        const float r0 = x0 * cs - x1 * sn, r1 = x0 * sn + x1 * cs;
-        x0 = r0;
-        x1 = r1;
+        sincos_far(((float)pos * a.esc) * freq, sn, cs);
+        if (l >= half) sn = 0.0f, cs = 1.0f;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const float r0 = x0[n] * cs - x1[n] * sn, r1 = x0[n] * sn + x1[n] * cs;
+            x0[n] = l < half ? r0 : x0[n];
+            x1[n] = l < half ? r1 : x1[n];
+        }
+        if (a.neox) {  // back to neighbouring channels
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                float* row = row_s[wave][n] + (lane - l) * 2;
+                row[i0] = x0[n];
+                row[i1] = x1[n];
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const float2 x = *reinterpret_cast<const float2*>(row_s[wave][n] + lane * 2);
+                x0[n] = x.x;
+                x1[n] = x.y;
+            }
+        }
     }
-    if (a.neox) {  // back to neighbouring channels
-        float* row = row_s[wave] + (lane - l) * 2;
-        row[i0] = x0;
-        row[i1] = x1;
-        __builtin_amdgcn_wave_barrier();
-        x0 = row[2 * l];
-        x1 = row[2 * l + 1];
-    }
-    // the largest magnitude of 32 channels (16 lanes; a NaN's or an infinity's bits lie above all others)
-    uint32_t m = max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu);
-    m = max(m, bfly<0>(m, lane));
-    m = max(m, bfly<1>(m, lane));
-    m = max(m, bfly<2>(m, lane));
-    m = max(m, bfly<3>(m, lane));
-    if (!on) return;
+    if (t >= T) return;
     const uint32_t c = 2 * l;
     if (isq) {
-        gstore<float2>(a.qo + 4ull * (((uint64_t)t * a.nh + h) * a.hd + c), make_float2(x0, x1));
+        const uint64_t out = a.qo + 4 * ((uint64_t)t0 * nx + h0) * HD;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+            if (h0 + n < nx) gstore<float2>(out + n * HD * 4 + (row0 + c) * 4, make_float2(x0[n], x1[n]));
         return;
     }
-    uint32_t slot = paso_pos(a.paso) + t;
+    uint32_t slot = pos0 + t;
     if (a.cap) slot %= a.cap;
     if (slot >= a.rows) return;
-    const uint32_t kvd = a.nkv * a.hd, ch = h * a.hd + c, R = mx_slots(a.rows);
-    if (a.fmt == 0) {
-        gstore<float2>((isv ? a.vc : a.kc) + 4 * ((uint64_t)slot * kvd + ch), make_float2(x0, x1));
-    } else if (a.fmt == 1) {
-        if (isv) {
-            mptr<uint16_t>(a.vc)[vt_index(slot, kvd, ch)] = f2h(x0);
-            mptr<uint16_t>(a.vc)[vt_index(slot, kvd, ch + 1)] = f2h(x1);
+    const uint32_t kvd = a.nkv * HD, R = mx_slots(a.rows);
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const uint32_t h = h0 + n, ch = h * HD + c;
+        if (h >= nx) break;
+        if (a.fmt == 0) {
+            gstore<float2>((isv ? a.vc : a.kc) + 4 * ((uint64_t)slot * kvd + ch), make_float2(x0[n], x1[n]));
+        } else if (a.fmt == 1) {
+            if (isv) {
+                mptr<uint16_t>(a.vc)[vt_index(slot, kvd, ch)] = f2h(x0[n]);
+                mptr<uint16_t>(a.vc)[vt_index(slot, kvd, ch + 1)] = f2h(x1[n]);
+            } else {
+                gstore<uint32_t>(a.kc + 2 * ((uint64_t)slot * kvd + ch), (uint32_t)f2h(x0[n]) | ((uint32_t)f2h(x1[n]) << 16));
+            }
         } else {
-            gstore<uint32_t>(a.kc + 2 * ((uint64_t)slot * kvd + ch), (uint32_t)f2h(x0) | ((uint32_t)f2h(x1) << 16));
-        }
-    } else {
-        const uint32_t x = mx_scale(__uint_as_float(m)), b0 = mx_byte(x0, x), b1 = mx_byte(x1, x);
-        if (isv) {
-            mptr<uint8_t>(a.vc)[mx_v_at(h, slot, c, R, a.hd)] = (uint8_t)b0;
-            mptr<uint8_t>(a.vc)[mx_v_at(h, slot, c + 1, R, a.hd)] = (uint8_t)b1;
-            if ((l & 15) == 0) mptr<uint8_t>(a.vc)[mx_vx_at(h, slot, l >> 4, R, a.hd, a.nkv)] = (uint8_t)x;
-        } else {
-            gstore<uint16_t>(a.kc + mx_k_at(h, slot, c, R, a.hd), (uint16_t)(b0 | (b1 << 8)));
-            if ((l & 15) == 0) mptr<uint8_t>(a.kc)[mx_kx_at(h, slot, l >> 4, R, a.hd, a.nkv)] = (uint8_t)x;
+            // the largest magnitude of 32 channels (16 lanes; a NaN's or an infinity's bits lie above all others)
+            uint32_t m = max(__float_as_uint(x0[n]) & 0x7fffffffu, __float_as_uint(x1[n]) & 0x7fffffffu);
+            m = max(m, bfly<0>(m, lane));
+            m = max(m, bfly<1>(m, lane));
+            m = max(m, bfly<2>(m, lane));
+            m = max(m, bfly<3>(m, lane));
+            const uint32_t x = mx_scale(__uint_as_float(m)), b0 = mx_byte(x0[n], x), b1 = mx_byte(x1[n], x);
+            if (isv) {
+                mptr<uint8_t>(a.vc)[mx_v_at(h, slot, c, R, HD)] = (uint8_t)b0;
+                mptr<uint8_t>(a.vc)[mx_v_at(h, slot, c + 1, R, HD)] = (uint8_t)b1;
+                if ((l & 15) == 0) mptr<uint8_t>(a.vc)[mx_vx_at(h, slot, l >> 4, R, HD, a.nkv)] = (uint8_t)x;
+            } else {
+                gstore<uint16_t>(a.kc + mx_k_at(h, slot, c, R, HD), (uint16_t)(b0 | (b1 << 8)));
+                if ((l & 15) == 0) mptr<uint8_t>(a.kc)[mx_kx_at(h, slot, l >> 4, R, HD, a.nkv)] = (uint8_t)x;
+            }
         }
     }
 }
+#define NORM_ROPE_KV(HD, N) \
+    KERNEL __launch_bounds__(256) void qp_norm_rope_kv_h##HD##_##N(QpRopeKvArgs a) { norm_rope_kv_body<HD, N>(a); }
+NORM_ROPE_KV(64, 1) NORM_ROPE_KV(64, 4) NORM_ROPE_KV(128, 1) NORM_ROPE_KV(128, 4)
 
 // ====================================================================================== reading back
 // Rows of positions p0 .. p0 + n - 1 as f32 or f16 [n][nkv hd]: a thread takes two channels of K and of V.

@@ -1080,7 +1080,12 @@ int op_norm_rope_kv(const Ctx& c) {
         if (n.p)
             if (int e = need_room(n.p, n.n, op, n.what)) return e;
     if (int e = kv_room(op, a.kc, a.vc, a.fmt, a.rows, a.nkv, a.hd)) return e;
-    return launch(K_norm_rope_kv, a.tcov, cdiv(a.nh + 2 * a.nkv, 512 / a.hd), 1, 256, 0, a);
+    // Four heads for each wavefront where one each would be twice what the device holds (8B shape, 512 tokens with their kv_read:
+    // 11.8 us, 12.2 with one; 2048: 27.5 and 31.3); else one (256 tokens: 8.6 us, 9.6 with four; 512 with heads of 64: 8.4, 8.7).
+    const bool h128 = a.hd == 128, four = (uint64_t)a.tcov * (a.nh + 2 * a.nkv) * a.hd / 128 >= 64ull * (g_cus > 0 ? g_cus : 1);
+    static const Kid k[2][2] = {{K_norm_rope_kv_h64_1, K_norm_rope_kv_h64_4}, {K_norm_rope_kv_h128_1, K_norm_rope_kv_h128_4}};
+    const uint32_t groups = four ? cdiv(a.nh, 4) + 2 * cdiv(a.nkv, 4) : a.nh + 2 * a.nkv;
+    return launch(k[h128][four], h128 ? a.tcov : cdiv(a.tcov, 2), cdiv(groups, 4), 1, 256, 0, a);
 }
 
 // kv_read: P{hd, nkv, cap, fmt, rows, p0, n, out}; [paso|0, kc, vc, k, v].  The rows of positions p0 .. p0 + n - 1 as f32
