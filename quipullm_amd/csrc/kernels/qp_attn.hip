@@ -255,10 +255,11 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
 #pragma unroll
         for (int r = 0; r < RG; r++) {
             const uint32_t bits = drafted(t, r);
+#pragma unroll 1
             for (uint32_t k = 0; k < 32; k++) {
                 if (!sees(t, r, k, bits)) continue;
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+                for (int d = 0; d < DT; d++) {
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
                         const uint32_t s = t.slot + k, c = kvh * HD + DT * (4 * g + x) + d;
@@ -266,6 +267,8 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
                                             : gload<float>(a.vc + 4 * ((uint64_t)s * kvd + c));
                         if (!(fabsf(v) < __builtin_inff())) o[r][d][x] = __builtin_nanf("");
                     }
+                    __builtin_amdgcn_sched_barrier(0);  // (a rare path: few registers before few waits)
+                }
             }
         }
 #pragma unroll

@@ -670,14 +670,16 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     bool alike = true;  // the lane's fit the f16 parts
 #pragma unroll
     for (int r = 0; r < RG; r++) {
+        const bool covered = w.r0 + r * 16 + n16 < w.nrow;  // (rows of the call past Paso's: anything may stand there)
         float v[KS][8], mine = 0.0f, least = 3.4e38f;  // the largest element, the least of the largest of 8 (not 0)
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const float4 x = qv[r][s][0], z = qv[r][s][1];
-            const float f[8] = {x.x, x.y, x.z, x.w, z.x, z.y, z.z, z.w};
+            float f[8] = {x.x, x.y, x.z, x.w, z.x, z.y, z.z, z.w};
             float eight = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
+                f[i] = covered ? f[i] : 0.0f;
                 const float u = fabsf(f[i]);
                 v[s][i] = a.scale < 0.0f ? -f[i] : f[i];
                 eight = fmaxf(eight, u);

@@ -1174,10 +1174,12 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     // 8-bit caches: blocks of 128 rows, whose wavefronts share the unpacked tiles, where there are enough of them for the
     // device's CUs, two on each where every share of the keys has 512 (8B shape, 2048 tokens: 108 us, 156 with blocks of 16
     // rows; 512 behind 8000: 158 and 213; a tree of 64 behind 32700: 90 and 115); else blocks of 16 rows (512 tokens without a
-    // past: 26 us, 38 with 128; 32 behind 480: 15 and 20).  f32 and f16 caches: 16 or 32 rows.
+    // past: 26 us, 38 with 128; 32 behind 480: 15 and 20).  f32 and
+    // f16 caches: 32 rows where a workgroup's 256 keys are work for each CU eight times over (tree of 64 behind 32000 keys of 4
+    // f16 heads: 175 us, 237 with 16 rows), else 16 (behind 4100 of 8 heads: 43, 46; tree of 25 behind 500: 10.2, 12.8).
     const uint64_t yw = (nrow + 127) / 128;
     const bool mx8 = fmt == QP_KV_MX8, wide = mx8 && nrow > 64 && (a.nkv * yw >= cus || a.nkv * yw * cdiv(keys, 512) >= 2 * cus);
-    const uint32_t RG = !mx8 && nrow > 16 ? 2 : 1, block = wide ? 128 : 16 * RG;
+    const uint32_t RG = !mx8 && a.nkv * cdiv(nrow, 32) * (uint64_t)cdiv(keys, 256) >= 8 * cus ? 2 : 1, block = wide ? 128 : 16 * RG;
     if ((nrow + block - 1) / block > 65535) return fail(QP_E_ARG, "%s: %u tokens in one call", op, T);
     const uint32_t yb = cdiv(nrow, block);
     const uint64_t per = (uint64_t)T * a.nh * (4 * a.hd + 8);  // bytes of one share's partial states
@@ -1187,11 +1189,13 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
         if (int e = need_room(parts, ns * per, op, "the shares' buffer")) return e;
         a.part_o = parts;
     } else if (!ns) {
-        // shares of 256 keys or more (512 in blocks of 128 rows), while they make at most two workgroups for each CU; none
-        // where the blocks alone are one for each (one token behind 4100 keys in 18 shares: 13.4 us, in 32 14.0)
+        // Shares of 256 keys or more (512 in blocks of 128 rows), while they make at most two workgroups for each CU; none
+        // where the blocks alone are one for each (one token behind 4100 keys in 18 shares: 13.4 us, in 32 14.0).  Up to 8
+        // shares may have 128 (32 tokens behind 480 keys: 11.3 us, 12.3 with two shares), unless all have 256 (25 tokens of a
+        // tree behind 96 keys: 7.8 us, 10.0 with two shares: their meeting costs 2 to 4).
         const uint32_t wgs = a.nkv * yb;
-        ns = wgs >= cus ? 1 : cdiv(2 * cus, wgs);
-        if (ns > cdiv(keys, wide ? 512 : 256)) ns = cdiv(keys, wide ? 512 : 256);
+        const uint32_t share = wide ? 512 : 256, few = keys <= 256 ? 1 : std::min(8u, std::min(cus / wgs, cdiv(keys, 128)));
+        ns = wgs >= cus ? 1 : std::max(few, std::min(cdiv(2 * cus, wgs), cdiv(keys, share)));
         if (ns > 64) ns = 64;
         if (g_capturing && !g_noalloc) ns = 1;
         if (g_noalloc && ns * per > QP_SCRATCH_BYTES) ns = 1;
