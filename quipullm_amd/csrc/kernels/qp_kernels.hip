@@ -4197,13 +4197,13 @@ QP_DEV void qp_dec_attn_comb_impl(QpDecCombArgs a) {
 
 // ====================================================================================== argmax
 // Greedy (reference sampling.js:38-42): strict '>' from -Infinity, so ties go to the lowest index and NaN is
-// never chosen.  Single workgroup.
+// never chosen.  One workgroup per row.
 KERNEL __launch_bounds__(1024) void qp_argmax(QpArgmaxArgs a) {
     __shared__ uint64_t wb[16];
     const uint32_t tid = threadIdx.x;
     uint64_t best = 0;
     for (uint32_t i = tid; i < a.n; i += 1024) {
-        const uint64_t k = amax_key(cptr<float>(a.v)[i], i);
+        const uint64_t k = amax_key(cptr<float>(a.v + 4ull * blockIdx.x * a.n)[i], i);
         best = k > best ? k : best;
     }
     for (int m = 32; m >= 1; m >>= 1) {
@@ -4215,7 +4215,7 @@ KERNEL __launch_bounds__(1024) void qp_argmax(QpArgmaxArgs a) {
     if (tid == 0) {
         uint64_t b = 0;
         for (int i = 0; i < 16; i++) b = wb[i] > b ? wb[i] : b;
-        mptr<uint32_t>(a.out)[0] = b ? 0xffffffffu - (uint32_t)(b & 0xffffffffu) : 0u;
+        mptr<uint32_t>(a.out)[blockIdx.x] = b ? 0xffffffffu - (uint32_t)(b & 0xffffffffu) : 0u;
     }
 }
 

@@ -1839,14 +1839,20 @@ int op_dec_attn_comb(const Ctx& c) {
     return launch(K_dec_attn_comb, a.nh, 1, 1, 256, 0, a);
 }
 
-// argmax: P{n}; [paso, v, out] (greedy, sampling.js:38-42).
+// argmax: P{n, rows}; [paso, v, out] (greedy, sampling.js:38-42).  rows 0 or 1: of v[n]; else out[r] of each row v[r][n].
 int op_argmax(const Ctx& c) {
     if (int e = need_bufs(c, 3, "argmax")) return e;
     QpArgmaxArgs a = {};
+    const uint32_t rows = c.U(1) ? c.U(1) : 1;
     a.n = c.U(0);
     a.v = c.B(1);
     a.out = c.B(2);
-    return launch(K_argmax, 1, 1, 1, 1024, 0, a);
+    if (rows > 1) {
+        if (rows > 65535) return fail(QP_E_ARG, "argmax: %u rows", rows);
+        if (int e = need_room(a.v, 4ull * rows * a.n, "argmax", "the rows")) return e;
+        if (int e = need_room(a.out, 4ull * rows, "argmax", "the output")) return e;
+    }
+    return launch(K_argmax, rows, 1, 1, 1024, 0, a);
 }
 
 // argmax_fin: P{count, advance, cap}; [paso, amax, ids, tokens|0, step].  cap = entries of tokens.

@@ -38,7 +38,7 @@ function args(argv) {
 }
 
 async function cargar(o) {
-  const options = { tiled_prefill: !o['no-tiled'], kv_f16: o.kv === 'f16' };
+  const options = { tiled_prefill: !o['no-tiled'], kv_f16: o.kv === 'f16', kv_mx8: o.kv === 'mx8' };
   if (o.batch) options.batch = parseInt(o.batch, 10);
   if (o['max-gen']) options.max_gen = parseInt(o['max-gen'], 10);
   if (o.eager) options.eager_decode = true;
@@ -74,8 +74,10 @@ async function generate(o) {
       const v = o[k.replace(/_/g, '-')];
       if (v !== undefined) params[k] = parseFloat(v);
     }
+    if (o.drafts) params.ramas = parseInt(o.drafts, 10);
     const r = await engine.generar(modelo, ids, params);
     for (const t of r.ids) toks.push(t);
+    if (r.ramas) extra.drafts = r.ramas;
   } else if (o.mode === 'sample') {
     if (!modelo.pasoMuestreado) throw new Error('this model has no fused one-token plan for the sampled mode');
     // sampled continuation on the fused one-token plan (device penalties and top-k candidates, host draw); each
@@ -218,7 +220,7 @@ async function bench(o) {
     if (P > ids.length) throw new Error('prompt file has ' + ids.length + ' ids, ' + P + ' requested');
     runs.push(await medir(modelo, ids, P, n, warm, !!o.eager, !!o.sample));
   }
-  const r = { runs: runs, load_ms: loadMs, ctx: modelo.ctx, nsplit: modelo.nsplit, kv_f16: modelo.kvF16,
+  const r = { runs: runs, load_ms: loadMs, ctx: modelo.ctx, nsplit: modelo.nsplit, kv_f16: modelo.kvF16, kv_mx8: modelo.kvMx8,
     batch: modelo.batch, bytes_on_gpu: modelo.gpu.bytesUsados, check_ids: check };
   modelo.free();
   process.stdout.write(JSON.stringify(r) + '\n');
@@ -227,7 +229,7 @@ async function bench(o) {
 // The engine of quipullm's server (motor.js): hello, then jobs from the long poll until the server says "cerrar".
 async function motor(o) {
   const { Motor } = require('./motor');
-  const opciones = { kv_f16: o.kv === 'f16' };
+  const opciones = { kv_f16: o.kv === 'f16', kv_mx8: o.kv === 'mx8' };
   if (o.batch) opciones.batch = parseInt(o.batch, 10);
   if (o['max-gen']) opciones.max_gen = parseInt(o['max-gen'], 10);
   if (o['keys-per-split']) opciones.attn_keys_per_split = parseInt(o['keys-per-split'], 10);

@@ -118,16 +118,20 @@ async function generar(modelo, ids, params) {
     if (params.alToken && await params.alToken(t, out.length)) { razon = 'stop'; return true; }
     return false;
   };
-  if (mu.esVoraz() && modelo.decodificarVoraz && !params.host_loop) {
+  // params.ramas: greedy with up to that many drafted tokens, looked up in the text so far, verified in each pass
+  const ramas = mu.esVoraz() && params.ramas > 0 && modelo.decodificarRamas && !params.host_loop;
+  const cuenta = {};
+  if (ramas || (mu.esVoraz() && modelo.decodificarVoraz && !params.host_loop)) {
     const primero = argmax(logits);
     if (esFin(primero)) razon = 'stop';
     else if (!(await emitir(primero))) {
       const resto = maxTok - 1;
-      const bloque = params.bloque || resto;
+      const bloque = params.bloque || (ramas ? 32 : resto);
       let hechos = 0;
       while (hechos < resto) {
         const n = Math.min(bloque, resto - hechos);
-        const nuevos = modelo.decodificarVoraz(out[out.length - 1], n);
+        const nuevos = ramas ? modelo.decodificarRamas(out[out.length - 1], n, { ramas: params.ramas, cuenta: cuenta }) :
+          modelo.decodificarVoraz(out[out.length - 1], n);
         let parar = false;
         for (const t of nuevos) {
           if (esFin(t)) { razon = 'stop'; parar = true; break; }
@@ -161,7 +165,7 @@ async function generar(modelo, ids, params) {
   const tEnd = Date.now();
   const seg = (tEnd - tPrompt) / 1000;
   return { ids: out, razon: razon, prompt_ms: tPrompt - t0, decode_ms: tEnd - tPrompt,
-    tps: out.length && seg > 0 ? out.length / seg : null, reutilizados: saltar };
+    tps: out.length && seg > 0 ? out.length / seg : null, reutilizados: saltar, ramas: ramas ? cuenta : undefined };
 }
 
 module.exports = { cargarRegistro: cargarRegistro, cargarModelo: cargarModelo, cargarDesdeMeta: cargarDesdeMeta,

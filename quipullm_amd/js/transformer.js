@@ -83,6 +83,10 @@ class ModeloTransformer {
     const op = meta.options || {};
     this.batch = op.batch || 32;                 // tokens per prefill pass (reference transformer.js:10 uses 32)
     this.kvF16 = !!op.kv_f16;                    // f16 KV cache (the reference keeps it in f32)
+    // 8-bit KV cache in blocks of 32 channels that share a power of two: norm_rope_kv writes it, atencion_mx8 reads it
+    this.kvMx8 = !!op.kv_mx8;
+    if (this.kvF16 && this.kvMx8) throw new Error('kv_f16 and kv_mx8: one cache type');
+    this.fmtKV = this.kvMx8 ? 2 : this.kvF16 ? 1 : 0;
     this.eagerDecode = !!op.eager_decode;        // fused step dispatched op by op instead of a captured graph
     // decode attention: keys per workgroup at full context: 256 (two 32-key tiles per wavefront) while that still
     // gives at least 64 workgroups (nkv x splits), else 128
@@ -200,16 +204,17 @@ class ModeloTransformer {
           capa.down = c.matriz(p + 'ffn_down.weight');
           F = Math.max(F, capa.gate.N);
         }
-        const kvd = this.nkv * this.hd, eb = this.kvF16 ? 2 : 4;
+        const kvd = this.nkv * this.hd, eb = this.kvF16 ? 2 : 4, r32 = (n) => Math.ceil(n / 32) * 32;
         // windowed layers keep a ring of window + batch slots (transformer.js:106-111): position p in slot p % cap
         // holds the window of every token of a batch as it is processed
         capa.swa = this.esSwa(i) ? this.ventana : 0;
         capa.anillo = capa.swa && this.ctx > capa.swa + this.batch ? capa.swa + this.batch : 0;
         capa.slots = capa.anillo || this.ctx;
-        capa.kc = gpu.buffer(capa.slots * kvd * eb, undefined, 'kcache' + i);
+        const mxBytes = r32(capa.slots) * kvd * 33 / 32;
+        capa.kc = gpu.buffer(this.kvMx8 ? mxBytes : capa.slots * kvd * eb, undefined, 'kcache' + i);
         // the f16 value cache is stored in whole tiles of 32 slots, read whole by the decode attention: it starts
         // zeroed so that slots not yet written hold finite values (they are weighted by 0)
-        const vBytes = (this.kvF16 ? Math.ceil(capa.slots / 32) * 32 : capa.slots) * kvd * eb;
+        const vBytes = this.kvMx8 ? mxBytes : (this.kvF16 ? r32(capa.slots) : capa.slots) * kvd * eb;
         capa.vc = gpu.buffer(vBytes, undefined, 'vcache' + i);
         if (!ceros || ceros.length < vBytes) ceros = new Uint8Array(vBytes);
         gpu.escribir(capa.vc, 0, ceros.subarray(0, vBytes));
@@ -277,6 +282,15 @@ class ModeloTransformer {
     }
     this.ropeFreq = B(4 * Math.max(1, this.nrot / 2), 'rope_freq');
     gpu.escribir(this.ropeFreq, 0, tablaRope(this.base, this.nrot));
+    // (the windowed layers' base: the table that norm_rope_kv takes there)
+    this.ropeFreqSwa = this.ropeFreq;
+    if (this.gemma && this.ventana && this.baseSwa !== this.base) {
+      this.ropeFreqSwa = B(4 * Math.max(1, this.nrot / 2), 'rope_freq_swa');
+      gpu.escribir(this.ropeFreqSwa, 0, tablaRope(this.baseSwa, this.nrot));
+    }
+    // 8-bit cache: the one-token step's shares of the keys (256 each at full context) and their partial states
+    this.nsMx8 = Math.max(1, Math.min(64, Math.ceil(this.ctx / 256)));
+    this.parteMx8 = this.kvMx8 && this.nsMx8 > 1 ? B(this.nsMx8 * this.nh * (4 * this.hd + 8), 'mx8_parts') : null;
     this.amax = B(8 * AMAX_WG, 'argmax_partials');
     gpu.escribir(this.amax, 0, new Uint8Array(8 * AMAX_WG));
     this.maxGen = op_max_gen(this.meta);
@@ -332,6 +346,22 @@ class ModeloTransformer {
     return gpu.grupo('embed_' + E.tipo, [u, this.bPaso].concat(wb, [ids, y]));
   }
 
+  // norm_rope_kv of layer c: Q and K normed and rotated, K and V into the cache.  pos: the tokens' positions (a tree's), or
+  // null for consecutive ones.
+  _guardar(c, pos) {
+    const swa = this.gemma && c.swa, esc = this.gemma && !c.swa ? this.escalaGlobal : 1;
+    return this.gpu.grupo('norm_rope_kv', [this.gpu.uniforme([['u', this.hd], ['u', this.nh], ['u', this.nkv], ['u', this.neox],
+      ['f', this.eps], ['u', this.nrot], ['f', esc], ['u', c.anillo], ['u', this.fmtKV], ['u', c.slots]]), this.bPaso, this.q,
+      this.k, this.v, this.q, c.kc, c.vc, c.qNorm || null, c.kNorm || null, swa ? this.ropeFreqSwa : this.ropeFreq, pos]);
+  }
+
+  // atencion_mx8 of layer c; parte: the buffer of `ns` shares of the keys, or null (the library's workspace).
+  _atencionMx8(c, ns, parte) {
+    return this.gpu.grupo('atencion_mx8', [this.gpu.uniforme([['u', this.hd], ['u', this.nh], ['u', this.nkv], ['u', c.swa],
+      ['f', this.escAtt], ['u', c.anillo], ['u', 0], ['u', 0], ['u', 2], ['u', c.slots], ['u', ns]]), this.bPaso, this.q, c.kc,
+      c.vc, this.att, parte]);
+  }
+
   _armarGrupos() {
     const gpu = this.gpu, D = this.D, P = this.bPaso;
     const G = {};
@@ -368,8 +398,10 @@ class ModeloTransformer {
         ropeK: gpu.grupo('norm_rope', [ur(this.nkv, !!c.kNorm), P, this.k, c.kNorm || dummy].concat(tablaCapa)),
         kvw: gpu.grupo('kv_write', [gpu.uniforme([['u', kvd], ['u', c.anillo], ['u', f16], ['u', c.slots]]), P, this.k, this.v,
           c.kc, c.vc]),
-        att: gpu.grupo('atencion', [gpu.uniforme([['u', this.hd], ['u', this.nh], ['u', this.nkv], ['u', c.swa],
-          ['f', this.escAtt], ['u', c.anillo], ['u', 0], ['u', 0], ['u', f16], ['u', c.slots]]), P, this.q, c.kc, c.vc, this.att]),
+        guardar: this.kvMx8 ? this._guardar(c, null) : null,
+        att: this.kvMx8 ? this._atencionMx8(c, 0, null) :
+          gpu.grupo('atencion', [gpu.uniforme([['u', this.hd], ['u', this.nh], ['u', this.nkv], ['u', c.swa],
+            ['f', this.escAtt], ['u', c.anillo], ['u', 0], ['u', 0], ['u', f16], ['u', c.slots]]), P, this.q, c.kc, c.vc, this.att]),
         wo: directo(c.wo, this.att, c.postAtt),
       };
       // the attention norm as input planes of Q, K and V (all K-quant, tiled)
@@ -433,6 +465,8 @@ class ModeloTransformer {
   reset() {
     this.pos = 0;   // the KV cache is overwritten by position (reference transformer.js:243-245)
     this.hist = [];
+    this.alto = 0;  // positions below it have been written since (drafted tokens' and dropped ids' among them)
+    this.rama = null;
   }
 
   // Prompt cache: how many leading ids of a new prompt are already in the KV cache (pos is set there), or 0 (the
@@ -446,7 +480,9 @@ class ModeloTransformer {
     while (n < m && h[n] === ids[n]) n++;
     // a ring of cap slots still holds the keys the recomputed positions need (from n + 1 - window on) only while
     // no later position has taken their slots: the history may not reach the first of them plus cap
-    for (const c of this.capas) if (c.anillo && h.length > Math.max(0, n + 1 - c.swa) + c.anillo) n = 0;
+    this.alto = Math.max(this.alto, h.length);
+    for (const c of this.capas) if (c.anillo && this.alto > Math.max(0, n + 1 - c.swa) + c.anillo) n = 0;
+    this.rama = null;
     h.length = n;
     this.pos = n;
     return n;
@@ -455,7 +491,8 @@ class ModeloTransformer {
   // The reference engine saves recurrent-state checkpoints here; a KV cache needs none.
   guardarPunto() {}
 
-  _despacharCapas(T) {
+  // arbol: the layers' groups of a drafted tree (_armarArbol) in place of the cache writes and the attention
+  _despacharCapas(T, arbol) {
     const G = this.G, self = this;
     const mm = function (g, uno) {
       if (uno === undefined) uno = T === 1;
@@ -472,7 +509,8 @@ class ModeloTransformer {
       if (d.norma) despachar(null, d.norma, T);
       despachar(null, d.suma, filas(self.D));
     };
-    for (const gc of G.capas) {
+    for (let i = 0; i < G.capas.length; i++) {
+      const gc = G.capas[i], ga = arbol ? arbol.capas[i] : gc;
       if (gc.attnNormPl && T >= 256) {
         despachar(null, gc.attnNormPl, Math.ceil(T / 8));
         mm(gc.wqPl); mm(gc.wkPl); mm(gc.wvPl);
@@ -480,14 +518,18 @@ class ModeloTransformer {
         despachar(null, gc.attnNorm, T);
         mm(gc.wq); mm(gc.wk); mm(gc.wv);
       }
-      despachar(null, gc.ropeQ, this.nh, T);
-      despachar(null, gc.ropeK, this.nkv, T);
-      despachar(null, gc.kvw, Math.ceil(T * this.nkv * this.hd / 256));
-      if (gc.attPl && T >= 256) {
+      if (ga.guardar) {
+        despachar(null, ga.guardar, this.nh, T);
+      } else {
+        despachar(null, gc.ropeQ, this.nh, T);
+        despachar(null, gc.ropeK, this.nkv, T);
+        despachar(null, gc.kvw, Math.ceil(T * this.nkv * this.hd / 256));
+      }
+      if (gc.attPl && T >= 256 && !arbol) {
         despachar(null, gc.attPl, this.nh, T);
         salida(gc.woPl);
       } else {
-        despachar(null, gc.att, this.nh, T);
+        despachar(null, ga.att, this.nh, T);
         salida(gc.wo);
       }
       const gluPl = !this.nExp && gc.gluPl && T >= 256;
@@ -529,6 +571,7 @@ class ModeloTransformer {
     if (this.pos + T > this.ctx) return Promise.reject(new Error('context exceeded (' + this.ctx + ' tokens)'));
     for (const id of ids) if (!(id >= 0 && id < this.vocab)) return Promise.reject(new Error('token id ' + id + ' outside the vocabulary'));
     const gpu = this.gpu;
+    this.rama = null;
     gpu.escribir(this.bPaso, 0, new Uint32Array([T, this.pos, 0, 0]));
     gpu.escribir(this.bIds, 0, new Uint32Array(ids));
     const mm = this._despacharCapas(T);
@@ -541,10 +584,140 @@ class ModeloTransformer {
     if (!conLogits) return Promise.resolve(null);
     const out = new Float32Array(this.vocab);
     gpu.leer(this.logits, 0, out);
-    // on the host, as the reference (transformer.js:333-334)
+    return Promise.resolve(this._ajustar(out));
+  }
+
+  // The logit scale and soft cap, on the host, as the reference (transformer.js:333-334).
+  _ajustar(out) {
     if (this.escLogit) { const k = 1 / this.escLogit; for (let i = 0; i < out.length; i++) out[i] *= k; }
     if (this.softcap) { const c = this.softcap; for (let i = 0; i < out.length; i++) out[i] = c * Math.tanh(out[i] / c); }
-    return Promise.resolve(out);
+    return out;
+  }
+
+  // ---------------------------------------------------------------- drafted trees
+  _armarArbol() {
+    if (this.arbol) return this.arbol;
+    const gpu = this.gpu, TB = this.batch, B = (n, l) => { const b = gpu.buffer(n, undefined, l); this.bufs.push(b); return b; };
+    const a = { mask: B(4 * TB * Math.ceil(TB / 32), 'tree_mask'), pos: B(4 * TB, 'tree_pos'), idx: B(4 * TB, 'tree_path'),
+      logits: B(4 * TB * this.vocab, 'tree_logits'), sig: B(4 * TB, 'tree_next') };
+    a.capas = this.capas.map((c) => ({
+      guardar: this._guardar(c, a.pos),
+      att: gpu.grupo('atencion_arbol', [gpu.uniforme([['u', this.hd], ['u', this.nh], ['u', this.nkv], ['u', c.swa],
+        ['f', this.escAtt], ['u', c.anillo], ['u', this.fmtKV], ['u', c.slots], ['u', 0]]), this.bPaso, this.q, c.kc, c.vc, this.att,
+        a.mask, a.pos, null]),
+    }));
+    a.norma = gpu.grupo('rmsnorm', [gpu.uniforme([['u', this.D], ['u', 0], ['f', this.eps], ['u', 0]]), this.bPaso, this.x,
+      this.normFinal, this.xn]);
+    a.salida = this._mm(this.salida, this.xn, a.logits, 0);
+    this.arbol = a;
+    return a;
+  }
+
+  // One pass over a tree of drafted tokens behind the processed ids, which stay as they are until aceptarRama: ids[i]
+  // follows ids[padres[i]], padres[i] < i, or the last processed id where padres[i] is -1.  Returns the model's greedy
+  // choice after each of them; opciones.logits(i, fila) gets each one's logits.
+  verificarArbol(ids, padres, opciones) {
+    const T = ids.length, W = Math.ceil(T / 32), gpu = this.gpu, op = opciones || {};
+    if (T < 1 || T > this.batch) throw new Error('a tree of 1 to ' + this.batch + ' tokens');
+    if (padres.length !== T) throw new Error('one parent for each token of the tree');
+    if (this.pos + T > this.ctx) throw new Error('context exceeded (' + this.ctx + ' tokens)');
+    for (const id of ids) if (!(id >= 0 && id < this.vocab)) throw new Error('token id ' + id + ' outside the vocabulary');
+    const mask = new Uint32Array(T * W), pos = new Uint32Array(T);
+    for (let i = 0; i < T; i++) {
+      const p = padres[i];
+      if (!Number.isInteger(p) || p < -1 || p >= i) throw new Error('token ' + i + ' of the tree follows token ' + p);
+      if (p >= 0) for (let w = 0; w < W; w++) mask[i * W + w] = mask[p * W + w];
+      mask[i * W + (i >> 5)] |= 1 << (i & 31);
+      pos[i] = p < 0 ? this.pos : pos[p] + 1;
+    }
+    const a = this._armarArbol();
+    this.rama = null;
+    gpu.escribir(this.bPaso, 0, new Uint32Array([T, this.pos, 0, 0]));
+    gpu.escribir(this.bIds, 0, new Uint32Array(ids));
+    gpu.escribir(a.mask, 0, mask);
+    gpu.escribir(a.pos, 0, pos);
+    const mm = this._despacharCapas(T, a);
+    despachar(null, a.norma, T);
+    mm(a.salida);
+    this.alto = Math.max(this.alto, this.hist.length, this.pos + T);
+    const sig = new Uint32Array(T);
+    if (op.logits || this.escLogit || this.softcap) {
+      // (the scale and the cap may make equal what was not: the choice is of the adjusted logits, as forward's)
+      const todo = new Float32Array(T * this.vocab);
+      gpu.leer(a.logits, 0, todo);
+      for (let i = 0; i < T; i++) {
+        const f = this._ajustar(todo.subarray(i * this.vocab, (i + 1) * this.vocab));
+        let m = 0;
+        for (let j = 1; j < f.length; j++) if (f[j] > f[m]) m = j;
+        sig[i] = m;
+        if (op.logits) op.logits(i, f);
+      }
+    } else {
+      despachar(null, gpu.grupo('argmax', [gpu.uniforme([['u', this.vocab], ['u', T]]), this.bPaso, a.logits, a.sig]), 1);
+      gpu.leer(a.sig, 0, sig);
+    }
+    this.rama = { ids: Array.from(ids), padres: Array.from(padres) };
+    return sig;
+  }
+
+  // The path camino (indexes of the tree of the last verificarArbol, each the parent of the next, the first one's parent
+  // -1) becomes part of the processed ids: its rows move to the positions behind them.
+  aceptarRama(camino) {
+    const r = this.rama, n = camino.length, gpu = this.gpu;
+    if (!r) throw new Error('no verified tree');
+    for (let i = 0; i < n; i++)
+      if (!(camino[i] < r.ids.length) || r.padres[camino[i]] !== (i ? camino[i - 1] : -1)) throw new Error('not a path of the tree');
+    if (camino.some((c, i) => c !== i)) {
+      gpu.escribir(this.arbol.idx, 0, new Uint32Array(camino));
+      const porTipo = new Map();   // caches of one size go together, up to 64 layers in a launch
+      for (const c of this.capas) {
+        const k = c.anillo + ' ' + c.slots;
+        if (!porTipo.has(k)) porTipo.set(k, []);
+        porTipo.get(k).push(c);
+      }
+      for (const l of porTipo.values())
+        for (let i = 0; i < l.length; i += 64) {
+          const u = gpu.uniforme([['u', this.hd], ['u', this.nkv], ['u', l[0].anillo], ['u', this.fmtKV], ['u', l[0].slots], ['u', n]]);
+          despachar(null, gpu.grupo('kv_ramal', [u, this.bPaso, this.arbol.idx].concat(
+            ...l.slice(i, i + 64).map((c) => [c.kc, c.vc]))), 1);
+        }
+    }
+    for (const c of camino) this.hist.push(r.ids[c]);
+    this.pos += n;
+    this.rama = null;
+  }
+
+  // Greedy continuation with drafts looked up in the processed ids: the ids that followed earlier occurrences of the last
+  // ones (up to 3) make a tree of at most opciones.ramas tokens, which one pass verifies; the path that the model agrees with
+  // is kept, with its own next choice.  Consumes `primero`, processes n ids and returns the n ids that follow them, as
+  // decodificarVoraz does.  opciones.cuenta, if given, counts {pasos, aceptados}.
+  decodificarRamas(primero, n, opciones) {
+    const op = opciones || {}, max = Math.min(this.batch, 1 + (op.ramas || 16)), out = [], cuenta = op.cuenta || {};
+    if (n < 1) return out;
+    if (this.pos + n > this.ctx) throw new Error('context exceeded (' + this.ctx + ' tokens)');
+    cuenta.pasos = cuenta.pasos || 0;
+    cuenta.aceptados = cuenta.aceptados || 0;
+    let t = primero;
+    while (out.length < n) {
+      const falta = n - out.length;
+      const a = arbolDe(this.hist.concat([t]), Math.min(max, this.ctx - this.pos), falta);
+      cuenta.pasos++;
+      if (a.ids.length === 1 && this.decodificarVoraz) {
+        out.push(this.decodificarVoraz(t, 1)[0]);
+      } else {
+        const sig = this.verificarArbol(a.ids, a.padres), camino = [0];
+        for (;;) {
+          const s = sig[camino[camino.length - 1]], hijo = a.hijo(camino[camino.length - 1], s);
+          out.push(s);
+          if (hijo < 0 || out.length === n) break;
+          camino.push(hijo);
+        }
+        cuenta.aceptados += camino.length - 1;
+        this.aceptarRama(camino);
+      }
+      t = out[out.length - 1];
+    }
+    return out;
   }
 
   // ---------------------------------------------------------------- fused greedy decode
@@ -655,7 +828,10 @@ class ModeloTransformer {
       } else {
       for (const g of this._gemvPorFormato([{ W: c.wq, mode: STORE, y: this.q }, { W: c.wk, mode: STORE, y: this.k },
         { W: c.wv, mode: STORE, y: this.v }], this.x, c.attnNorm, D)) plan.push([g, 1]);
-      if (this.atencionUnida) {
+      if (this.kvMx8) {
+        plan.push([gc.guardar, [this.nh, 1, 1]]);
+        plan.push([this._atencionMx8(c, this.nsMx8, this.parteMx8), [this.nh, 1, 1]]);
+      } else if (this.atencionUnida) {
         this.usaMerged = true;
         plan.push([gpu.grupo('dec_attn', [uAttM, P, this.q, this.k, this.v, c.kc, c.vc, c.qNorm, c.kNorm, this.partO,
           this.partML, this.ropeFreq, this.att, this.attCnt]), 1]);
@@ -768,6 +944,7 @@ class ModeloTransformer {
     if (!(primero >= 0 && primero < this.vocab)) throw new Error('token id ' + primero + ' outside the vocabulary');
     this.prepararDecode();
     const gpu = this.gpu;
+    this.rama = null;
     gpu.escribir(this.bPaso, 0, new Uint32Array([1, this.pos, 0, 0]));
     gpu.escribir(this.bIds, 0, new Uint32Array([primero]));
     gpu.escribir(this.contador, 0, new Uint32Array([0, 0, 0, 0]));
@@ -817,6 +994,7 @@ class ModeloTransformer {
     if (!(id >= 0 && id < this.vocab)) throw new Error('token id ' + id + ' outside the vocabulary');
     this.prepararDecode();
     const gpu = this.gpu;
+    this.rama = null;
     gpu.escribir(this.bPaso, 0, new Uint32Array([1, this.pos, 0, 0]));
     gpu.escribir(this.bIds, 0, new Uint32Array([id]));
     this._pasos(1);
@@ -890,7 +1068,8 @@ class ModeloTransformer {
   }
 
   // The KV cache as this backend holds it, for checking against the CPU oracle: per layer the K cache bytes then
-  // the V cache bytes ([ctx][kvd] f32 or f16 rows; the f16 V cache in its 32-slot tiles), written to `ruta`.
+  // the V cache bytes ([ctx][kvd] f32 or f16 rows; the f16 V cache in its 32-slot tiles; 8-bit caches in theirs), written
+  // to `ruta`.
   volcarKV(ruta) {
     const fs = require('fs');
     const fd = fs.openSync(ruta, 'w');
@@ -922,9 +1101,37 @@ function tablaRope(base, nrot) {
   return t;
 }
 
+// A tree of drafted tokens for the ids `h`: its root is the last of them; below it, what followed the earlier occurrences of
+// the last 3, then 2, then 1 ids, the most recent first, at most max tokens in all and `largo` below the root.
+function arbolDe(h, max, largo) {
+  const N = h.length, ids = [h[N - 1]], padres = [-1], hijos = [new Map()];
+  for (let g = Math.min(3, N - 1); g >= 1 && ids.length < max; g--) {
+    for (let j = N - 2; j >= g - 1 && ids.length < max; j--) {
+      let igual = true;
+      for (let k = 0; k < g && igual; k++) igual = h[j - k] === h[N - 1 - k];
+      if (!igual) continue;
+      let nodo = 0;
+      for (let k = j + 1; k < N && k - j < largo; k++) {
+        let hijo = hijos[nodo].get(h[k]);
+        if (hijo === undefined) {
+          if (ids.length === max) break;
+          hijo = ids.length;
+          ids.push(h[k]);
+          padres.push(nodo);
+          hijos.push(new Map());
+          hijos[nodo].set(h[k], hijo);
+        }
+        nodo = hijo;
+      }
+    }
+    if (ids.length > 1) break;   // (shorter matches only where the longer ones gave nothing)
+  }
+  return { ids: ids, padres: padres, hijo: function (i, id) { const x = hijos[i].get(id); return x === undefined ? -1 : x; } };
+}
+
 function op_max_gen(meta) {
   const op = meta.options || {};
   return op.max_gen || 4096;
 }
 
-module.exports = { ModeloTransformer: ModeloTransformer, tablaRope: tablaRope, agrupable: agrupable };
+module.exports = { ModeloTransformer: ModeloTransformer, tablaRope: tablaRope, agrupable: agrupable, arbolDe: arbolDe };
