@@ -317,7 +317,8 @@ constexpr float MX_LOG2E = 1.4426950408889634f;
 //
 // Probabilities are 2^(s - m) with a reference m of the row that lies MX_UP below its largest score, so that their f16 parts
 // stay normal.  m follows the largest score only when a tile passes it by MX_LAG: until then probabilities of up to
-// 2^(MX_UP + MX_LAG) are summed as they are, and no wavefront exchanges maxima or rescales its outputs.
+// 2^(MX_UP + MX_LAG) are summed as they are, and no wavefront exchanges maxima or rescales its outputs.  (Where 2^20 is past, m
+// is the largest score itself: less 10 it could be rounded to 16 or 32 below, and a probability to 2^16, past f16's range.)
 constexpr float MX_LAG = 5.0f, MX_UP = 10.0f;
 
 // What a wavefront works on.  WIDE: a workgroup takes 128 RG (query, head) rows of one KV head, 16 RG for each of its eight
@@ -464,7 +465,7 @@ struct MxState {
             mx[r] = s[r][0][0];
 #pragma unroll
             for (int j = 1; j < 8; j++) mx[r] = fmaxf(mx[r], s[r][j >> 2][j & 3]);
-            past = past | (mx[r] * c[r] > m[r] + (MX_UP + MX_LAG));
+            past = past | (fmaf(mx[r], c[r], -m[r]) > MX_UP + MX_LAG);  // (m + 15 may be rounded to the next 16)
         }
         if (__any(past)) {
             bool b = false;
@@ -472,7 +473,8 @@ struct MxState {
             for (int r = 0; r < RG; r++) {
                 mx[r] = fmaxf(mx[r], bfly_f<4>(mx[r], w.lane));
                 mx[r] = fmaxf(mx[r], bfly_f<5>(mx[r], w.lane));
-                const float mn = fmaxf(m[r], mx[r] * c[r] - MX_UP), f = __builtin_amdgcn_exp2f(m[r] - mn);
+                const float top = mx[r] * c[r], mn = fmaxf(m[r], top - (fabsf(top) > 0x1p20f ? 0.0f : MX_UP));
+                const float f = __builtin_amdgcn_exp2f(m[r] - mn);
                 m[r] = mn;
                 l[r] *= f;
 #pragma unroll

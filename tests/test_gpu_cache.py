@@ -534,3 +534,61 @@ def test_one_share_while_capturing(quipu, dev):
             assert np.array_equal(dev.get(o, (1, nh, hd)), want)
     finally:
         quipu.graph_free(g)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("power", [19, 20, 21, 22, 23, 24, 25, 26, 27, 28, 40])
+def test_scores_past_their_last_place(quipu, dev, power, wide):
+    """Scores around 2^power, in units of log2, that grow by 15.5 from tile to tile, where the sum of a score and a few units is
+    rounded by more than a unit.  Each tile has one key whose score is not -2^power.  A row's largest score leads the others by
+    15.5 less the rounding of both (2^-22 of 2^power together: two sums of products, two products with the unit), so that its
+    key's value is the output up to 2^(that - 15.5) (1 + 2^-15) of two values' difference."""
+    hd, nh, nkv = 128, 32 if wide else 4, 8 if wide else 1
+    T, n = (256, 4224) if wide else (1, 160)
+    pos0 = n - T
+    rng = np.random.default_rng(power)
+    k, v = np.zeros((n, nkv, hd)), rng.standard_normal((n, nkv, hd)).astype(np.float32)
+    q = np.zeros((T, nh, hd), np.float32)
+    per = np.sqrt(hd) * np.log(2.0)  # q k of one unit of log2
+    tile = np.arange(n) // 32
+    # three blocks of channels: 2^power, then 15.5 for each tile of 64, then 15.5 for each 64 tiles
+    q[..., 0], q[..., 32], q[..., 64] = 2.0 ** (power - 14) * per, 15.5 * per, 15.5 * per
+    k[:, :, 0], k[:, :, 32], k[:, :, 64] = -(2.0 ** 14), (tile % 64)[:, None], 64 * (tile // 64)[:, None]
+    k[5::32, :, 0] = 2.0 ** 14
+    kc, vc, _, held = mx8.cache(mx8.MX8, k, v)
+    o, _ = run_attention(quipu, dev, q, kc, vc, T, pos0, nkv, mx8.MX8, n)
+    last = (pos0 + np.arange(T) - 5) // 32 * 32 + 5  # the last key with a score that the token sees
+    want = held[last][:, np.arange(nh) * nkv // nh]
+    most = np.abs(held).max()
+    off = 2.0 ** (power - 22)
+    if off < 15:
+        assert np.all(np.abs(o - want) <= 2.0 ** (off - 15.5) * 1.01 * 2 * most + 1e-5), np.abs(o - want).max()
+    assert np.isfinite(o).all() and np.abs(o).max() <= most * (1 + 1e-5)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T", [1, 40])
+def test_keys_and_queries_in_the_thousands(quipu, dev, T, fmt):
+    """Scores up to 1e9, as the keys and queries of some models make them: nearly one key for each row.  A score is off by 2^-20
+    of the sum of its products' magnitudes; rows whose two largest differ by less are within the values, and not compared."""
+    hd, nh, nkv, n = 128, 8, 2, 500
+    rng = np.random.default_rng(T)
+    q = (rng.standard_normal((T, nh, hd)) * 5000).astype(np.float32)
+    k, v = rng.standard_normal((n, nkv, hd)) * 5000, rng.standard_normal((n, nkv, hd)) * 1000
+    kc, vc, kh, vh = mx8.cache(fmt, k, v)
+    see = causal(T, n - T, 0, n)
+    mask = np.zeros((T, (T + 31) // 32), np.uint32)
+    for t in range(T):
+        for j in range(t + 1):
+            mask[t, j // 32] |= np.uint32(1 << (j % 32))
+    o, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, fmt, n, mask=mask)
+    want = mx8.attend(q.astype(np.float64), kh, vh, see, scale)
+    kk = np.repeat(kh, nh // nkv, 1)
+    scores = np.einsum("thc,nhc->thn", q.astype(np.float64), kk) * scale
+    size = np.einsum("thc,nhc->thn", np.abs(q).astype(np.float64), np.abs(kk)) * scale
+    top = np.sort(np.where(see[:, None], scores, -np.inf), -1)
+    clear = top[..., -1] - top[..., -2] > size.max() * 2.0 ** -20 + 20
+    assert clear.mean() > 0.9
+    most = np.abs(vh).max()
+    assert np.all(np.abs(o - want)[clear] <= 1e-5 * most)
+    assert np.isfinite(o).all() and np.abs(o).max() <= most * (1 + 1e-5)
