@@ -35,7 +35,7 @@ int g_device = 0;
 hipStream_t g_stream = nullptr;
 hipModule_t g_mod = nullptr;  // the first code object (timeline builds read its records)
 std::mutex g_mu;
-std::unordered_map<uint64_t, uint64_t> g_allocs;  // address -> bytes
+std::map<uint64_t, uint64_t> g_allocs;  // address -> bytes
 uint64_t g_bytes = 0;
 bool g_capturing = false;
 bool g_noalloc = false;    // inside qp_dispatch_noalloc: the prefill workspace is the fixed scratch array
@@ -1161,6 +1161,7 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     const uint32_t T = c.gy ? c.gy : 1, G = a.nh / a.nkv;
     if (a.cap && (!a.swa || (uint64_t)a.swa + T - 1 > a.cap))
         return fail(QP_E_ARG, "%s: a ring of %u slots does not hold a window of %u for %u tokens", op, a.cap, a.swa, T);
+    if (a.swa >> 31) return fail(QP_E_ARG, "%s: a window of %u keys", op, a.swa);
     if (!a.paso || !a.q || !a.o) return fail(QP_E_ARG, "%s: null binding", op);
     const uint64_t r32 = ((uint64_t)a.rows + 31) / 32 * 32;
     const uint64_t reach = fmt == QP_KV_MX8 ? r32 * a.hd : r32 * a.nkv * a.hd * (fmt == QP_KV_F16 ? 2 : 4);
@@ -1433,9 +1434,10 @@ int op_moe_comb(const Ctx& c) {
 
 // Bytes from p to the end of the library buffer that holds it (0: not inside one).
 uint64_t buf_room(uint64_t p) {
-    for (const auto& kv : g_allocs)
-        if (p >= kv.first && p < kv.first + kv.second) return kv.first + kv.second - p;
-    return 0;
+    auto it = g_allocs.upper_bound(p);
+    if (it == g_allocs.begin()) return 0;
+    --it;
+    return p - it->first < it->second ? it->first + it->second - p : 0;
 }
 
 // moe_group (kds.js:491-516): P{E, n}; [paso, sel, lst, off].  lst[off[e] .. off[e+1]) = the jobs
