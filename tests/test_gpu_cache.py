@@ -592,3 +592,101 @@ def test_keys_and_queries_in_the_thousands(quipu, dev, T, fmt):
     most = np.abs(vh).max()
     assert np.all(np.abs(o - want)[clear] <= 1e-5 * most)
     assert np.isfinite(o).all() and np.abs(o).max() <= most * (1 + 1e-5)
+
+
+def sampled(rng, T, most=20):
+    """Some of T rows: the first, the last, those at the edges of blocks, others."""
+    edges = [x for x in (0, 1, 15, 16, 31, 32, 33, T // 2, T - 2, T - 1) if 0 <= x < T]
+    return np.unique(np.concatenate([edges, rng.integers(0, T, most - 10)])).astype(int)
+
+
+@pytest.mark.parametrize("hd,nh,nkv,T,pos0,swa,cap", [
+    (128, 32, 8, 256, 4200, 0, 0),      # blocks of 128 rows and shares of the keys
+    (128, 32, 8, 1100, 0, 0, 0),        # blocks of 128 rows, the last with 48, no shares
+    (64, 24, 8, 1500, 37, 0, 0),        # groups of 3 heads: blocks that begin inside a token
+    (64, 32, 8, 1100, 3000, 300, 1500), # a ring
+    (128, 16, 16, 700, 9000, 1024, 0),  # a window, no ring, shares
+    (128, 12, 4, 90, 9000, 0, 0),       # blocks of 16 rows, many shares
+])
+def test_attention_over_many_blocks(quipu, dev, hd, nh, nkv, T, pos0, swa, cap):
+    """As test_attention, the rows of some tokens, where launches are large."""
+    rng = np.random.default_rng(19)
+    n = pos0 + T
+    rows = cap or n + 9
+    q = rng.standard_normal((T, nh, hd)).astype(np.float32)
+    k, v = (rng.standard_normal((n, nkv, hd)) * 10.0 ** rng.uniform(-2, 1, (n, 1, 1)) for _ in "kv")
+    kc, vc, _, _ = mx8.cache(MX8, *ring_rows(k, v, n, pos0, swa, cap, rows, np.nan))
+    kh, vh = (mx8.dequantise(*mx8.quantise(x.astype(np.float32))) for x in (k, v))
+    some = sampled(rng, T)
+    see = causal(T, pos0, swa, n)[some]
+    for noalloc in (False, True):
+        got, scale = run_attention(quipu, dev, q, kc, vc, T, pos0, nkv, MX8, rows, swa, cap, noalloc=noalloc)
+        assert np.all(np.abs(got[some] - mx8.attend(q[some], kh, vh, see, scale)) <= bound(q[some], kh, vh, see, scale)), noalloc
+        assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,nh,nkv,T,pos0,swa,cap", [
+    (128, 32, 8, 128, 8200, 0, 0),      # 512 rows: blocks of 128 (8 bits), of 32 (f32, f16), shares
+    (64, 16, 16, 300, 9000, 600, 0),    # a window, ten words of mask
+])
+def test_tree_over_many_blocks(quipu, dev, hd, nh, nkv, T, pos0, swa, cap, fmt):
+    """As test_tree, the rows of some tokens, where launches are large."""
+    rng = np.random.default_rng(20)
+    n = pos0 + T
+    rows = n + 5
+    q = rng.standard_normal((T, nh, hd)).astype(np.float32)
+    k, v = (rng.standard_normal((n, nkv, hd)) for _ in "kv")
+    mask, drafts, depth = random_tree(rng, T, True)
+    where = pos0 + depth
+    some = sampled(rng, T)
+    see = np.zeros((T, n), bool)
+    see[:, pos0:] = drafts
+    see[:, :pos0] = (np.arange(pos0)[None] > (where - swa)[:, None]) if swa else True
+    for bad in (False, True):
+        if bad:  # a drafted token whose value is not finite, seen by few
+            v[pos0 + T // 3, :, 5::64] = np.inf
+        kc, vc, _, _ = mx8.cache(fmt, *ring_rows(k, v, n, pos0, swa, cap, rows, np.nan))
+        if not bad:
+            held = [mx8.cache(fmt, x, x)[2] for x in (k, v)]
+        got, scale = run_attention(quipu, dev, q, kc, vc, T, pos0, nkv, fmt, rows, swa, cap, mask, where)
+        want, lim = mx8.attend(q[some], *held, see[some], scale), bound(q[some], *held, see[some], scale)
+        hit = see[:, pos0 + T // 3] & bad
+        assert np.all(np.abs(got[some] - want)[~hit[some]] <= lim[~hit[some]])
+        assert np.isfinite(got[~hit]).all() and not np.isfinite(got[hit][..., 5::64]).any()
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("T,cover,pos0", [(3, 40, 200), (1, 2, 0), (100, 300, 4000)])
+def test_rows_past_the_tokens_may_hold_anything(quipu, dev, T, cover, pos0, tree):
+    """A call for `cover` tokens of which the Paso has T: the queries behind them are NaN, and their outputs stay as they were."""
+    hd, nh, nkv, n = 128, 16, 4, pos0 + T
+    rng = np.random.default_rng(21)
+    q = np.full((cover, nh, hd), np.nan, np.float32)
+    q[:T] = rng.standard_normal((T, nh, hd))
+    k, v = (rng.standard_normal((n, nkv, hd)) for _ in "kv")
+    kc, vc, kh, vh = mx8.cache(MX8, k, v)
+    rows = pos0 + cover + 9
+    pad = lambda x: np.concatenate([x, np.zeros((rows - n, nkv, hd))])   # noqa: E731
+    grown = mx8.cache(MX8, pad(k), pad(v))[:2]
+    mask = np.zeros((cover, (cover + 31) // 32), np.uint32)
+    for t in range(cover):
+        for j in range(t + 1):
+            mask[t, j // 32] |= np.uint32(1 << (j % 32))
+    got, scale = run_attention(quipu, dev, q, *grown, T, pos0, nkv, MX8, rows, mask=mask if tree else None, cover=cover)
+    see = causal(T, pos0, 0, n)
+    assert np.all(np.abs(got[:T] - mx8.attend(q[:T], kh, vh, see, scale)) <= bound(q[:T], kh, vh, see, scale))
+    assert np.all(got[T:] == 9.0)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7])
+@pytest.mark.parametrize("n", [1, 1000, 128256])
+def test_argmax_of_rows(quipu, dev, rows, n):
+    rng = np.random.default_rng(n)
+    v = rng.standard_normal((rows, n)).astype(np.float32)
+    v[:, n // 2] = v[:, n - 1] = 9.0   # ties: the lowest index
+    v[:, 0] = np.nan if n > 1 else v[:, 0]
+    out = dev.buf(np.full(rows + 1, 77, np.uint32))
+    quipu.dispatch("argmax", [("u", n), ("u", rows)], [0, dev.buf(v), out])
+    got = dev.get(out, (rows + 1,), np.uint32)
+    assert got[:rows].tolist() == [n // 2] * rows and got[rows] == 77
