@@ -1116,7 +1116,8 @@ int op_kv_read(const Ctx& c) {
     if (int e = need_room(a.v, bytes, op, "the values' rows")) return e;
     if (int e = kv_room(op, a.kc, a.vc, a.fmt, a.rows, a.nkv, a.hd)) return e;
     if (!a.n) return 0;
-    return launch(K_kv_read, grid_cap((uint64_t)a.n * a.nkv * a.hd / 2), 1, 1, 256, 0, a);
+    const uint32_t pairs = a.nkv * a.hd / 2, hold = pairs >= 256 ? 1 : 256 / pairs;
+    return launch(K_kv_read, cdiv(pairs, 256), std::min(cdiv(a.n, hold), 65535u), 1, 256, 0, a);
 }
 
 // kv_ramal: P{hd, nkv, cap, fmt, rows, n}; [paso, idx, kc, vc of each layer ...] (up to 64 layers).  The rows of drafted
