@@ -52,7 +52,8 @@ typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 
 // TREE (atencion_arbol): the T rows are drafted tokens of a tree behind pos0 keys.  All of them see those keys (from their
 // window on), and of the drafted keys those that their mask names.  A value that is not finite reaches the rows that see its
-// key and no others (without TREE: every row of the block), and a row that sees no key is 0.
+// key and no others (without TREE: every row of the block), and a row that sees no key is 0.  A tree of 8 behind 4100 keys of
+// 8 f16 heads: 13.8 us and 4.3 for the shares' meeting (17 MB: latency); of 64 behind 32000 of 4: 175 us with RG 2, 237 with 1.
 template <int HD, bool F16, int RG, bool TREE = false>
 QP_DEV void attn_x_body(const QpAttnArgs& a) {
     constexpr int KS = HD / 32, DT = HD / 16;  // steps of 32 dimensions, tiles of 16 (DT dimensions per lane of 16)
