@@ -351,7 +351,8 @@ struct MxWork {
     QP_DEV MxWork(const QpAttnArgs& args) : a(args) {
         lane = threadIdx.x & 63, g = lane >> 4, n16 = lane & 15;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        G = a.nh / a.nkv, kvh = blockIdx.x, R = mx_slots(a.rows);
+        G = a.group, kvh = blockIdx.x, R = mx_slots(a.rows);
+        hk = (uint64_t)kvh * R * HD, hx = (uint64_t)a.nkv * R * HD + (uint64_t)kvh * R * NB;
         // long prompts: the blocks with the most keys first, then those with the fewest on (two workgroups share a CU)
         const uint32_t y = blockIdx.y, ny = gridDim.y, blk = TREE ? y : y < (ny + 1) / 2 ? ny - 1 - y : y - (ny + 1) / 2;
         b0 = blk * (WIDE ? 128 * RG : 16 * RG);
@@ -362,11 +363,11 @@ struct MxWork {
         const uint2 paso = gload<uint2>(a.paso);
         T = min(__builtin_amdgcn_readfirstlane(paso.x), a.tcov), pos0 = __builtin_amdgcn_readfirstlane(paso.y), nrow = T * G;
         if (b0 >= nrow) return false;
-        b_lo = b0 / G, b_hi = (min(b0 + (WIDE ? 128 * RG : 16 * RG), nrow) - 1) / G;
-        t_lo = min(r0, nrow - 1) / G, t_hi = (min(r0 + 16 * RG, nrow) - 1) / G;
+        b_lo = token(b0), b_hi = token(min(b0 + (WIDE ? 128 * RG : 16 * RG), nrow) - 1);
+        t_lo = token(min(r0, nrow - 1)), t_hi = token(min(r0 + 16 * RG, nrow) - 1);
 #pragma unroll
         for (int r = 0; r < RG; r++) {
-            const uint32_t t = row(r) / G;
+            const uint32_t t = token(row(r));
             uint32_t p = pos0 + t;
             if constexpr (TREE) {
                 if (a.where) p = min(max(cptr<uint32_t>(a.where)[t], pos0), pos0 + T - 1);
@@ -382,16 +383,17 @@ struct MxWork {
         const uint32_t nkey = a.cap ? min(kend - kbeg, a.cap) : kend - kbeg;
         end_a = a.cap ? min(first + nkey, a.cap) : first + nkey, end_b = first + nkey - end_a;
         ta = nkey ? (end_a + 31) / 32 - first / 32 : 0;
-        const uint32_t nt = ta + (end_b + 31) / 32, per = (nt + a.nsplit - 1) / a.nsplit;
+        const uint32_t nt = ta + (end_b + 31) / 32, per = a.nsplit_inv ? __umulhi(nt + a.nsplit - 1, a.nsplit_inv) : nt;
         i0 = blockIdx.z * per, i1 = min(nt, i0 + per);
-        hk = (uint64_t)kvh * R * HD, hx = (uint64_t)a.nkv * R * HD + (uint64_t)kvh * R * NB;
         return true;
     }
+    // the token of (query, head) row x (below 2^23)
+    QP_DEV uint32_t token(uint32_t x) const { return a.group_inv ? __umulhi(x, a.group_inv) : x; }
     // the lane's row of group r (past those that the dispatch covers: the last), and its query from the lane's inputs on
     QP_DEV uint32_t row(int r) const { return min(r0 + r * 16 + n16, a.tcov * G - 1); }
     QP_DEV uint64_t query(int r) const {
-        const uint32_t rc = row(r);
-        return a.q + 4 * (((uint64_t)(rc / G) * a.nh + kvh * G + rc % G) * HD + 16 * g);
+        const uint32_t rc = row(r), t = token(rc);
+        return a.q + 4 * (((uint64_t)t * a.nh + kvh * G + rc - t * G) * HD + 16 * g);
     }
     QP_DEV Tile tile(uint32_t i) const {
         if (i < ta) return {(first / 32 + i) * 32, first, end_a, (int)(kbeg - first)};
@@ -427,7 +429,8 @@ struct MxWork {
     }
     // Channels c .. c + 3 of (query, head) row `row` from its state (m, l): the output, or this share's partial state.
     QP_DEV void put(uint32_t row, uint32_t c, float4 s, float m, float l) const {
-        const uint64_t at = (uint64_t)(row / G) * a.nh + kvh * G + row % G;
+        const uint32_t t = token(row);
+        const uint64_t at = (uint64_t)t * a.nh + kvh * G + row - t * G;
         if (a.nsplit == 1) {
             const float f = l == 0.0f ? 0.0f : 1.0f / l;  // (l = 0: no key seen, and s = 0)
             gstore<float4>(a.o + 4 * (at * HD + c), make_float4(s.x * f, s.y * f, s.z * f, s.w * f));
@@ -633,7 +636,8 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     extern __shared__ float4 mx_lds[];
     W w(a);
     // The queries' loads do not wait for the Paso, the first tiles' not for the queries (one token behind 4100 keys: 9.4 us,
-    // 10.0 with each after the other).
+    // 10.0 with each after the other), nor for the Paso where neither a window nor shares put them anywhere but at the start (one
+    // token behind 100 keys: 7.0 us, 7.3).
     float4 qv[RG][KS][2];
 #pragma unroll
     for (int r = 0; r < RG; r++) {
@@ -643,41 +647,49 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
 #pragma unroll
             for (int i = 0; i < 2; i++) qv[r][s][i] = gload<float4>(at + (s >> 1) * 256 + (s & 1) * 32 + i * 16);
     }
-    if (!w.begin()) return;
-    const uint32_t lane = w.lane, g = w.g, n16 = w.n16, wave = w.wave, i1 = w.i1;
+    const uint32_t lane = w.lane, g = w.g, n16 = w.n16, wave = w.wave;
     const float scale = fabsf(a.scale) * MX_LOG2E;
     const __amdgpu_buffer_rsrc_t kr = kq_rsrc(a.kc + w.hk, (uint64_t)w.R * HD), vr = kq_rsrc(a.vc + w.hk, (uint64_t)w.R * HD);
     const __amdgpu_buffer_rsrc_t kxr = kq_rsrc(a.kc + w.hx, (uint64_t)w.R * NB), vxr = kq_rsrc(a.vc + w.hx, (uint64_t)w.R * NB);
+    constexpr uint32_t NONE = 0xffffffffu;
     uint32_t kx[2], vx[2];  // the scales of the lane's key of each half, and of its 8 values' keys
-    auto load_kx = [&](uint32_t i) __attribute__((always_inline)) {
+    auto load_kx = [&](uint32_t slot) __attribute__((always_inline)) {  // (of a tile at `slot`; none: NONE)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const uint32_t x = i < i1 ? (w.tile(i).slot + h * 16 + n16) * NB : QP_NOOFF;
+            const uint32_t x = slot != NONE ? (slot + h * 16 + n16) * NB : QP_NOOFF;
             if constexpr (NB == 4) kx[h] = __builtin_amdgcn_raw_buffer_load_b32(kxr, x, 0, 0);
             else kx[h] = __builtin_amdgcn_raw_buffer_load_b16(kxr, x, 0, 0);
         }
     };
-    auto load_vx = [&](uint32_t i) __attribute__((always_inline)) {
-        const auto x = __builtin_amdgcn_raw_buffer_load_b64(vxr, i < i1 ? w.tile(i).slot * NB + (n16 * DT / 32) * 32 + g * 8 : QP_NOOFF, 0, 0);
+    auto load_vx = [&](uint32_t slot) __attribute__((always_inline)) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b64(vxr, slot != NONE ? slot * NB + (n16 * DT / 32) * 32 + g * 8 : QP_NOOFF, 0, 0);
         vx[0] = x[0];
         vx[1] = x[1];
     };
     u32x4 kw[2 * CC], vw[DT / 2];  // not WIDE: the wavefront's tile
-    auto load_k = [&](uint32_t i) __attribute__((always_inline)) {
-        const uint32_t o = i < i1 ? w.tile(i).slot * HD + lane * 16 : QP_NOOFF;
-        load_kx(i);
+    auto load_k = [&](uint32_t slot) __attribute__((always_inline)) {
+        const uint32_t o = slot != NONE ? slot * HD + lane * 16 : QP_NOOFF;
+        load_kx(slot);
 #pragma unroll
         for (int c = 0; c < 2 * CC; c++) kw[c] = __builtin_amdgcn_raw_buffer_load_b128(kr, o, c * 1024, 0);
     };
-    auto load_v = [&](uint32_t i) __attribute__((always_inline)) {
-        const uint32_t o = i < i1 ? w.tile(i).slot * HD + lane * 16 : QP_NOOFF;
-        load_vx(i);
+    auto load_v = [&](uint32_t slot) __attribute__((always_inline)) {
+        const uint32_t o = slot != NONE ? slot * HD + lane * 16 : QP_NOOFF;
+        load_vx(slot);
 #pragma unroll
         for (int c = 0; c < DT / 2; c++) vw[c] = __builtin_amdgcn_raw_buffer_load_b128(vr, o, c * 1024, 0);
     };
-    if constexpr (!WIDE) {
-        load_k(w.i0 + wave);
-        load_v(w.i0 + wave);
+    const bool ahead = !WIDE && a.nsplit == 1 && !a.swa && wave * 32 < w.R;
+    if (ahead) {
+        load_k(wave * 32);
+        load_v(wave * 32);
+    }
+    if (!w.begin()) return;
+    const uint32_t i1 = w.i1;
+    auto slot_of = [&](uint32_t i) __attribute__((always_inline)) { return i < i1 ? w.tile(i).slot : NONE; };
+    if (!WIDE && !ahead) {
+        load_k(slot_of(w.i0 + wave));
+        load_v(slot_of(w.i0 + wave));
     }
     // ---- the rows' queries
     h8 qh[RG][KS], ql[RG][KS];
@@ -891,7 +903,7 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
                     scores(s, 2 * c + u, unpack8(kw[c][2 * u], kw[c][2 * u + 1], f, off),
                            unpack8(kw[CC + c][2 * u], kw[CC + c][2 * u + 1], f1, off1));
             }
-            load_k(i + 4);
+            load_k(slot_of(i + 4));
             float c[RG];
             st.follow(w, t, s, cs, c);
             st.weigh(s, c);
@@ -903,7 +915,7 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
 #pragma unroll
             for (int d = 0; d < DT; d += 2)
                 outputs(d, unpack8(vw[d >> 1][0], vw[d >> 1][1], f, off), unpack8(vw[d >> 1][2], vw[d >> 1][3], f, off));
-            load_v(i + 4);
+            load_v(slot_of(i + 4));
         }
         ok = __syncthreads_and(ok) != 0;
     } else {
@@ -966,8 +978,8 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
                 if (settle_now) {
                     __syncthreads();
                     load(i);
-                    load_kx(i);
-                    load_vx(i);
+                    load_kx(slot_of(i));
+                    load_vx(slot_of(i));
                     clear_k(t);
                     clear_v(t);
                     ok = settle_k() && settle_v(t);  // (the same in all wavefronts: they see the same scales)

@@ -201,7 +201,10 @@ typedef struct {
     // atencion_arbol: mask [T][mw] words, bit j % 32 of word j / 32 of row t: token t sees drafted token j (slot pos0 + j);
     // where: 0, or the tokens' positions [T] (pos0 .. pos0 + T - 1), from which windows count
     uint64_t mask, where;
-    uint32_t mw, pad;
+    uint32_t mw;
+    // atencion_mx8, atencion_arbol: nh / nkv, and ceil(2^32 / it), ceil(2^32 / nsplit) (0 for 1): x / d is the high word of the
+    // product for x below 2^32 / d
+    uint32_t group, group_inv, nsplit_inv;
 } QpAttnArgs;
 
 // ---------------------------------------------------------------- 8-bit caches, drafted trees (qp_cache.hip)

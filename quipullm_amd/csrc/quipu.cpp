@@ -1209,6 +1209,9 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     a.f16 = fmt;
     a.tcov = T;
     a.nsplit = ns;
+    a.group = G;
+    a.group_inv = G > 1 ? cdiv(1ull << 32, G) : 0;
+    a.nsplit_inv = ns > 1 ? cdiv(1ull << 32, ns) : 0;
     a.part_ml = ns > 1 ? a.part_o + 4ull * T * a.nh * ns * a.hd : 0;
     static const Kid k8[2][2][2] = {{{K_attn_mx8_h64_causal, K_attn_mx8_h64_causal_wide}, {K_attn_mx8_h128_causal, K_attn_mx8_h128_causal_wide}},
                                     {{K_attn_mx8_h64_tree, K_attn_mx8_h64_tree_wide}, {K_attn_mx8_h128_tree, K_attn_mx8_h128_tree_wide}}};
