@@ -1073,20 +1073,24 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
         QpAttnArgs a) { attn_mx8_body<HD, 1, TREE, true>(a); }
 ATTN_MX8(64, causal, false) ATTN_MX8(128, causal, false) ATTN_MX8(64, tree, true) ATTN_MX8(128, tree, true)
 
-// The shares' partial states of each (query, head) row -> o, in their order: grid rows, hd threads (at most 64 shares).
-// A row that no share saw a key of is 0.  4 us for 18 shares of 32 rows, 7.7 for 64.  (Joined by the last workgroup of the
+// The shares' partial states of each (query, head) row -> o, in a fixed order: grid rows, NY hd threads (at most 64 shares), the NY
+// threads of one channel dealing the shares out.  A row that no share saw a key of is 0.  64 shares of 32 rows: 5.3 us (one
+// thread for each channel: 7.7); 4 shares of 1024 rows: 3.9 (four threads: 4.4).  (Joined by the last workgroup of the
 // attention's own launch instead, through counters: one token behind 4100 keys 13.2 us, 12.6 with this launch; 8 tokens 20.3 and
 // 15.5, since that workgroup joins 16 rows; with fences that write back the L2 in place of stores through it 19.4 and 35.6.)
-KERNEL __launch_bounds__(128) void qp_attn_mx8_comb(QpAttnArgs a) {
-    __shared__ float wt[64], den;
-    const uint32_t t = blockIdx.x / a.nh, d = threadIdx.x, ns = a.nsplit, T = paso_T(a.paso);
+template <uint32_t NY>
+QP_DEV void attn_mx8_comb(const QpAttnArgs& a) {
+    __shared__ float wt[64], den, sum[NY][128];
+    const uint32_t t = blockIdx.x / a.nh, d = NY == 1 ? threadIdx.x : threadIdx.x & (a.hd - 1);
+    const uint32_t y = NY == 1 ? 0 : threadIdx.x / a.hd;
+    const uint32_t ns = a.nsplit, T = paso_T(a.paso);
     const uint64_t row = blockIdx.x, po = a.part_o + 4 * (row * ns * a.hd + d);
     float v[8];
 #pragma unroll
-    for (uint32_t s = 0; s < 8; s++) v[s] = s < ns ? gload<float>(po + 4ull * s * a.hd) : 0.0f;
-    const float2 mine = d < ns ? gload<float2>(a.part_ml + 8 * (row * ns + d)) : make_float2(-3.0e38f, 0.0f);
+    for (uint32_t s = 0; s < 8; s++) v[s] = NY * s + y < ns ? gload<float>(po + 4ull * (NY * s + y) * a.hd) : 0.0f;
+    const float2 mine = threadIdx.x < ns ? gload<float2>(a.part_ml + 8 * (row * ns + threadIdx.x)) : make_float2(-3.0e38f, 0.0f);
     if (t >= T) return;  // (the loads above are of the buffer all the same)
-    if (d < 64) {
+    if (threadIdx.x < 64) {
         const float M = wave_max_v(mine.x, d), f = mine.y != 0.0f ? __builtin_amdgcn_exp2f(mine.x - M) : -1.0f;
         wt[d] = f;
         const float L = wave_sum_v(mine.y != 0.0f ? mine.y * f : 0.0f, d);
@@ -1094,12 +1098,20 @@ KERNEL __launch_bounds__(128) void qp_attn_mx8_comb(QpAttnArgs a) {
     }
     __syncthreads();
     float o = 0.0f;
-    for (uint32_t s0 = 0; s0 < ns; s0 += 8) {
+    for (uint32_t s0 = y; s0 < ns; s0 += 8 * NY) {
 #pragma unroll
         for (uint32_t s = 0; s < 8; s++)
-            if (s0 + s < ns && wt[s0 + s] != -1.0f) o += v[s] * wt[s0 + s];
+            if (s0 + NY * s < ns && wt[s0 + NY * s] != -1.0f) o += v[s] * wt[s0 + NY * s];
 #pragma unroll
-        for (uint32_t s = 0; s < 8; s++) v[s] = s0 + 8 + s < ns ? gload<float>(po + 4ull * (s0 + 8 + s) * a.hd) : 0.0f;
+        for (uint32_t s = 0; s < 8; s++) v[s] = s0 + NY * (8 + s) < ns ? gload<float>(po + 4ull * (s0 + NY * (8 + s)) * a.hd) : 0.0f;
+    }
+    if constexpr (NY == 4) {
+        sum[y][d] = o;
+        __syncthreads();
+        if (y) return;
+        o = (o + sum[1][d]) + (sum[2][d] + sum[3][d]);
     }
     gstore<float>(a.o + 4 * (row * a.hd + d), den == 0.0f ? 0.0f : o / den);
 }
+KERNEL __launch_bounds__(128) void qp_attn_mx8_comb(QpAttnArgs a) { attn_mx8_comb<1>(a); }
+KERNEL __launch_bounds__(512) void qp_attn_mx8_comb4(QpAttnArgs a) { attn_mx8_comb<4>(a); }

@@ -1220,7 +1220,9 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     const Kid k = mx8 ? k8[tree][a.hd == 128][wide] : kt[fmt][a.hd == 128][RG == 2];
     const uint32_t lds = wide ? 2 * 128 * a.hd + 16 : 4 * RG * 16 * (a.hd + 4) * 4 + 4 * RG * 16 * 8;
     if (int e = launch(k, a.nkv, yb, ns, wide ? 512 : 256, lds, a)) return e;
-    return ns == 1 ? 0 : launch(K_attn_mx8_comb, T * a.nh, 1, 1, a.hd, 0, a);
+    if (ns == 1) return 0;
+    // (a thread has the loads of 8 shares in flight: past those, four threads for each channel)
+    return ns > 8 ? launch(K_attn_mx8_comb4, T * a.nh, 1, 1, 4 * a.hd, 0, a) : launch(K_attn_mx8_comb, T * a.nh, 1, 1, a.hd, 0, a);
 }
 
 // atencion_mx8: atencion over an 8-bit cache: P{hd, nh, nkv, swa, escala, cap, 0, 0, 2, rows, nsplit}; [paso, q, kc, vc, o,

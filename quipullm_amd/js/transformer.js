@@ -82,6 +82,7 @@ class ModeloTransformer {
     if (this.nh % this.nkv || this.nh / this.nkv > 8) throw new Error('GQA group ' + this.nh + '/' + this.nkv + ' not supported');
     const op = meta.options || {};
     this.batch = op.batch || 32;                 // tokens per prefill pass (reference transformer.js:10 uses 32)
+    this.maxArbol = Math.min(this.batch, 128);   // drafted tokens per verificarArbol (their logits stay on the device)
     this.kvF16 = !!op.kv_f16;                    // f16 KV cache (the reference keeps it in f32)
     // 8-bit KV cache in blocks of 32 channels that share a power of two: norm_rope_kv writes it, atencion_mx8 reads it
     this.kvMx8 = !!op.kv_mx8;
@@ -597,7 +598,7 @@ class ModeloTransformer {
   // ---------------------------------------------------------------- drafted trees
   _armarArbol() {
     if (this.arbol) return this.arbol;
-    const gpu = this.gpu, TB = this.batch, B = (n, l) => { const b = gpu.buffer(n, undefined, l); this.bufs.push(b); return b; };
+    const gpu = this.gpu, TB = this.maxArbol, B = (n, l) => { const b = gpu.buffer(n, undefined, l); this.bufs.push(b); return b; };
     const a = { mask: B(4 * TB * Math.ceil(TB / 32), 'tree_mask'), pos: B(4 * TB, 'tree_pos'), idx: B(4 * TB, 'tree_path'),
       logits: B(4 * TB * this.vocab, 'tree_logits'), sig: B(4 * TB, 'tree_next') };
     a.capas = this.capas.map((c) => ({
@@ -618,7 +619,7 @@ class ModeloTransformer {
   // choice after each of them; opciones.logits(i, fila) gets each one's logits.
   verificarArbol(ids, padres, opciones) {
     const T = ids.length, W = Math.ceil(T / 32), gpu = this.gpu, op = opciones || {};
-    if (T < 1 || T > this.batch) throw new Error('a tree of 1 to ' + this.batch + ' tokens');
+    if (T < 1 || T > this.maxArbol) throw new Error('a tree of 1 to ' + this.maxArbol + ' tokens');
     if (padres.length !== T) throw new Error('one parent for each token of the tree');
     if (this.pos + T > this.ctx) throw new Error('context exceeded (' + this.ctx + ' tokens)');
     for (const id of ids) if (!(id >= 0 && id < this.vocab)) throw new Error('token id ' + id + ' outside the vocabulary');
@@ -692,7 +693,7 @@ class ModeloTransformer {
   // is kept, with its own next choice.  Consumes `primero`, processes n ids and returns the n ids that follow them, as
   // decodificarVoraz does.  opciones.cuenta, if given, counts {pasos, aceptados}.
   decodificarRamas(primero, n, opciones) {
-    const op = opciones || {}, max = Math.min(this.batch, 1 + (op.ramas || 16)), out = [], cuenta = op.cuenta || {};
+    const op = opciones || {}, max = Math.min(this.maxArbol, 1 + (op.ramas || 16)), out = [], cuenta = op.cuenta || {};
     if (n < 1) return out;
     if (this.pos + n > this.ctx) throw new Error('context exceeded (' + this.ctx + ' tokens)');
     cuenta.pasos = cuenta.pasos || 0;

@@ -188,7 +188,7 @@ def test_shares_and_blocks(lib):
         return Call(lib, "atencion_mx8", T=T, hd=128, nh=nh, nkv=nkv, rows=rows, **kw).run()[1]
     assert [l[0] for l in shape(1, 200)] == ["qp_attn_mx8_h128_causal"]
     a = shape(1, 4400)
-    assert [l[0] for l in a] == ["qp_attn_mx8_h128_causal", "qp_attn_mx8_comb"] and a[0][1:] == ["8", "1", "18", "256"]
+    assert [l[0] for l in a] == ["qp_attn_mx8_h128_causal", "qp_attn_mx8_comb4"] and a[0][1:] == ["8", "1", "18", "256"]
     assert shape(1, 131072)[0][3] == "64"
     assert [l[0] for l in shape(2048, 2048)] == ["qp_attn_mx8_h128_causal_wide"]
     assert shape(512, 512)[0][:4] == ["qp_attn_mx8_h128_causal", "8", "128", "1"]
