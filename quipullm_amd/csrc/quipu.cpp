@@ -1174,13 +1174,15 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     const uint32_t cus = g_cus > 0 ? (uint32_t)g_cus : 1u;
     const uint64_t nrow = (uint64_t)T * G, keys = a.swa && (uint64_t)a.swa + T < a.rows ? a.swa + T : a.rows;
     // 8-bit caches: blocks of 128 rows, whose wavefronts share the unpacked tiles, where there are enough of them for the
-    // device's CUs, two on each where every share of the keys has 512 (8B shape, 2048 tokens: 108 us, 156 with blocks of 16
-    // rows; 512 behind 8000: 158 and 213; a tree of 64 behind 32700: 90 and 115); else blocks of 16 rows (512 tokens without a
-    // past: 26 us, 38 with 128; 32 behind 480: 15 and 20).  f32 and
-    // f16 caches: 32 rows where a workgroup's 256 keys are work for each CU eight times over (tree of 64 behind 32000 keys of 4
-    // f16 heads: 175 us, 237 with 16 rows), else 16 (behind 4100 of 8 heads: 43, 46; tree of 25 behind 500: 10.2, 12.8).
+    // device's CUs, five for two of them where every share of the keys has 512 (8B shape, 2048 tokens: 107 us, 151 with blocks
+    // of 16 rows; 1000: 51 and 54; 512 behind 8000: 158 and 213; a tree of 64 behind 32700: 88 and 115); else blocks of 16 rows
+    // (700 tokens behind 700: 60 us, 67 with 128; 500 without a past: 24 and 36; 32 behind 480: 15 and 20).  Blocks of 64 rows
+    // between the two (four wavefronts that share the unpacking) were nowhere faster: 52, 68 and 29 us for those of 1000, 700
+    // and 500.
+    // f32 and f16 caches: 32 rows where a workgroup's 256 keys are work for each CU eight times over (tree of 64 behind 32000
+    // keys of 4 f16 heads: 175 us, 237 with 16 rows), else 16 (behind 4100 of 8 heads: 43, 46; tree of 25 behind 500: 10.2, 12.8).
     const uint64_t yw = (nrow + 127) / 128;
-    const bool mx8 = fmt == QP_KV_MX8, wide = mx8 && nrow > 64 && (a.nkv * yw >= cus || a.nkv * yw * cdiv(keys, 512) >= 2 * cus);
+    const bool mx8 = fmt == QP_KV_MX8, wide = mx8 && nrow > 64 && (a.nkv * yw >= cus || 2 * a.nkv * yw * cdiv(keys, 512) >= 5 * cus);
     const uint32_t RG = !mx8 && a.nkv * cdiv(nrow, 32) * (uint64_t)cdiv(keys, 256) >= 8 * cus ? 2 : 1, block = wide ? 128 : 16 * RG;
     if ((nrow + block - 1) / block > 65535) return fail(QP_E_ARG, "%s: %u tokens in one call", op, T);
     const uint32_t yb = cdiv(nrow, block);

@@ -191,6 +191,8 @@ def test_shares_and_blocks(lib):
     assert [l[0] for l in a] == ["qp_attn_mx8_h128_causal", "qp_attn_mx8_comb4"] and a[0][1:] == ["8", "1", "18", "256"]
     assert shape(1, 131072)[0][3] == "64"
     assert [l[0] for l in shape(2048, 2048)] == ["qp_attn_mx8_h128_causal_wide"]
+    assert [l[0] for l in shape(256, 5556)] == ["qp_attn_mx8_h128_causal_wide", "qp_attn_mx8_comb"]
+    assert shape(700, 1400)[0][0] == "qp_attn_mx8_h128_causal"
     assert shape(512, 512)[0][:4] == ["qp_attn_mx8_h128_causal", "8", "128", "1"]
     c = Call(lib, "atencion_mx8", T=1, nh=32, nkv=8, rows=4400)
     parts, short = (lib.buf(n * 32 * (4 * 128 + 8)) for n in (7, 6))

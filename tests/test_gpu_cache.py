@@ -601,7 +601,8 @@ def sampled(rng, T, most=20):
 
 
 @pytest.mark.parametrize("hd,nh,nkv,T,pos0,swa,cap", [
-    (128, 32, 8, 256, 4200, 0, 0),      # blocks of 128 rows and shares of the keys
+    (128, 32, 8, 256, 4200, 0, 0),      # blocks of 16 rows
+    (128, 32, 8, 256, 5300, 0, 0),      # blocks of 128 rows and shares of the keys
     (128, 32, 8, 1100, 0, 0, 0),        # blocks of 128 rows, the last with 48, no shares
     (64, 24, 8, 1500, 37, 0, 0),        # groups of 3 heads: blocks that begin inside a token
     (64, 32, 8, 1100, 3000, 300, 1500), # a ring
@@ -627,7 +628,7 @@ def test_attention_over_many_blocks(quipu, dev, hd, nh, nkv, T, pos0, swa, cap):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("hd,nh,nkv,T,pos0,swa,cap", [
-    (128, 32, 8, 128, 8200, 0, 0),      # 512 rows: blocks of 128 (8 bits), of 32 (f32, f16), shares
+    (128, 32, 8, 128, 10400, 0, 0),     # 512 rows: blocks of 128 (8 bits), of 32 (f32, f16), shares
     (64, 16, 16, 300, 9000, 600, 0),    # a window, ten words of mask
 ])
 def test_tree_over_many_blocks(quipu, dev, hd, nh, nkv, T, pos0, swa, cap, fmt):
