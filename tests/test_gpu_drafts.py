@@ -217,3 +217,42 @@ def test_looked_up_drafts_give_the_greedy_ids(models_dir, tmp_path, name, kv):
     assert a["ids"] == b["ids"]
     assert a["pos"] == b["pos"] == len(prompt) + 39
     assert b["drafts"]["pasos"] + b["drafts"]["aceptados"] == 39
+
+
+RINGS = r"""
+const engine = require(%(eng)s);
+(async () => {
+  const p = %(p)s, x = %(x)s, path = %(path)s, op = {ctx: 256, options: {batch: 32}};
+  const gen = (m, ids, n) => engine.generar(m, ids, {temperature: 0, max_tokens: n});
+  const m = await engine.cargarModelo(path, op);
+  await gen(m, p, 10);                                     // positions 0 .. 68 written
+  const b = await gen(m, p.slice(0, 45).concat(x), 1);     // 45 of them stay
+  const c = await gen(m, p.slice(0, 20).concat(x), 10);    // position 0's slot has held position 56
+  await gen(m, p.slice(0, 30), 1);
+  const antes = m.alto;
+  m.verificarArbol(x.concat(x, x, x).slice(0, 28), new Array(28).fill(-1));   // positions 30 .. 57 written
+  const despues = m.alto;
+  const d = await gen(m, p.slice(0, 20).concat(x), 10);
+  m.free();
+  const f = await engine.cargarModelo(path, {ctx: 256, options: {batch: 32, prompt_cache: false}});
+  const c2 = await gen(f, p.slice(0, 20).concat(x), 10);
+  f.free();
+  console.log(JSON.stringify({b: b.reutilizados, c: c.reutilizados, d: d.reutilizados, cids: c.ids, dids: d.ids, want: c2.ids,
+    antes: antes, despues: despues}));
+})().catch((e) => { console.error(e.stack); process.exit(1); });
+"""
+
+
+def test_rings_remember_what_was_overwritten(models_dir):
+    """Ring caches (windows of 24, rings of 56 slots): a prefix is not reused where a position written since then, by ids that
+    were dropped or by drafted tokens, took the slot of a key that its window needs, though the ids processed now are few."""
+    path = synth.ensure_model("mini_gemma3_q4km_c", models_dir)
+    p, x = ([int(t) for t in synth.random_prompt(1000, n, s)] for n, s in ((60, 41), (7, 42)))
+    print("node rings", flush=True)
+    rc, o, err = run(["timeout", "-k", "5", "110", "node", "-e", RINGS % {k: json.dumps(v) for k, v in
+                                                                        dict(eng=ENG, p=p, x=x, path=path).items()}], timeout=120)
+    assert rc == 0, err[-3000:]
+    r = json.loads(o.strip().splitlines()[-1])
+    assert r["b"] == 45 and r["c"] == 0 and r["d"] == 0
+    assert r["cids"] == r["dids"] == r["want"]
+    assert r["despues"] == 58 and r["antes"] < 56
