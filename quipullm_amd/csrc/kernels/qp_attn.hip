@@ -507,7 +507,9 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
             const bool none = TREE && L == 0.0f;
             gstore<float4>(a.o + 4 * (at * HD + 4 * c), none ? make_float4(0, 0, 0, 0) : make_float4(s.x / L, s.y / L, s.z / L, s.w / L));
         } else {
-            gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + 4 * c), s);
+            // (TREE: met by qp_attn_mx8_comb, which takes outputs)
+            const float n = !TREE ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+            gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + 4 * c), make_float4(s.x * n, s.y * n, s.z * n, s.w * n));
             if (c == 0) gstore<float2>(a.part_ml + 8 * (at * a.nsplit + blockIdx.z), make_float2(M, L));
         }
     }

@@ -427,13 +427,13 @@ struct MxWork {
         const int k0 = (int)t.slot + t.off;
         return r0 < nrow && (TREE || (k0 <= (int)(pos0 + t_hi) && (!a.swa || k0 + 31 > (int)(pos0 + t_lo) - (int)a.swa)));
     }
-    // Channels c .. c + 3 of (query, head) row `row` from its state (m, l): the output, or this share's partial state.
+    // Channels c .. c + 3 of (query, head) row `row`, over the keys of the state (m, l): the output, or this share's partial
+    // state.  (States hold outputs that are divided by their l: o itself can be 2^15 times as large, past f32's range.)
     QP_DEV void put(uint32_t row, uint32_t c, float4 s, float m, float l) const {
         const uint32_t t = token(row);
         const uint64_t at = (uint64_t)t * a.nh + kvh * G + row - t * G;
         if (a.nsplit == 1) {
-            const float f = l == 0.0f ? 0.0f : 1.0f / l;  // (l = 0: no key seen, and s = 0)
-            gstore<float4>(a.o + 4 * (at * HD + c), make_float4(s.x * f, s.y * f, s.z * f, s.w * f));
+            gstore<float4>(a.o + 4 * (at * HD + c), s);
         } else {
             gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + c), s);
             if (c == 0) gstore<float2>(a.part_ml + 8 * (at * a.nsplit + blockIdx.z), make_float2(m, l));
@@ -550,9 +550,11 @@ struct MxState {
             l[r] += bfly_f<5>(l[r], lane);
         }
     }
-    QP_DEV float4 out4(int r, int x, int d, int back) const {  // channels DT (4 g + x) + d .. d + 3, times 2^back
-        return make_float4(__builtin_ldexpf(o[r][d][x], back), __builtin_ldexpf(o[r][d + 1][x], back),
-                           __builtin_ldexpf(o[r][d + 2][x], back), __builtin_ldexpf(o[r][d + 3][x], back));
+    // channels DT (4 g + x) + d .. d + 3, times 2^back, over l (no key seen: l = 0, o = 0)
+    QP_DEV float4 out4(int r, int x, int d, int back) const {
+        const float f = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+        return make_float4(__builtin_ldexpf(o[r][d][x] * f, back), __builtin_ldexpf(o[r][d + 1][x] * f, back),
+                           __builtin_ldexpf(o[r][d + 2][x] * f, back), __builtin_ldexpf(o[r][d + 3][x] * f, back));
     }
     template <class W>
     QP_DEV void put_all(const W& w, int back) const {
@@ -1048,18 +1050,21 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
             float M = -3.0e38f;
 #pragma unroll
             for (int v = 0; v < 4; v++) M = fmaxf(M, ml[2 * (v * RG * 16 + lr)]);
-            float L = 0.0f;
+            float f[4], L = 0.0f;  // the wavefronts' weights
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const float lw = ml[2 * (v * RG * 16 + lr) + 1];
+                f[v] = lw != 0.0f ? lw * __builtin_amdgcn_exp2f(ml[2 * (v * RG * 16 + lr)] - M) : 0.0f;
+                L += f[v];
+            }
+            const float n = L == 0.0f ? 0.0f : 1.0f / L;
             float4 s = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int v = 0; v < 4; v++) {
-                const uint32_t at = v * RG * 16 + lr;
-                const float lw = ml[2 * at + 1];
-                if (lw != 0.0f) {
-                    const float f = __builtin_amdgcn_exp2f(ml[2 * at] - M);
-                    const float4 x = *reinterpret_cast<const float4*>(ol + at * LD + c);
-                    L += lw * f;
-                    s = make_float4(s.x + x.x * f, s.y + x.y * f, s.z + x.z * f, s.w + x.w * f);
-                }
+                if (ml[2 * (v * RG * 16 + lr) + 1] == 0.0f) continue;  // (it saw no key)
+                const float4 x = *reinterpret_cast<const float4*>(ol + (v * RG * 16 + lr) * LD + c);
+                const float g = f[v] * n;
+                s = make_float4(s.x + x.x * g, s.y + x.y * g, s.z + x.z * g, s.w + x.w * g);
             }
             w.put(row, c, s, M, L);
         }
@@ -1080,7 +1085,7 @@ ATTN_MX8(64, causal, false) ATTN_MX8(128, causal, false) ATTN_MX8(64, tree, true
 // 15.5, since that workgroup joins 16 rows; with fences that write back the L2 in place of stores through it 19.4 and 35.6.)
 template <uint32_t NY>
 QP_DEV void attn_mx8_comb(const QpAttnArgs& a) {
-    __shared__ float wt[64], den, sum[NY][128];
+    __shared__ float wt[64], sum[NY][128];
     const uint32_t t = blockIdx.x / a.nh, d = NY == 1 ? threadIdx.x : threadIdx.x & (a.hd - 1);
     const uint32_t y = NY == 1 ? 0 : threadIdx.x / a.hd;
     const uint32_t ns = a.nsplit, T = paso_T(a.paso);
@@ -1091,10 +1096,9 @@ QP_DEV void attn_mx8_comb(const QpAttnArgs& a) {
     const float2 mine = threadIdx.x < ns ? gload<float2>(a.part_ml + 8 * (row * ns + threadIdx.x)) : make_float2(-3.0e38f, 0.0f);
     if (t >= T) return;  // (the loads above are of the buffer all the same)
     if (threadIdx.x < 64) {
-        const float M = wave_max_v(mine.x, d), f = mine.y != 0.0f ? __builtin_amdgcn_exp2f(mine.x - M) : -1.0f;
-        wt[d] = f;
-        const float L = wave_sum_v(mine.y != 0.0f ? mine.y * f : 0.0f, d);
-        if (d == 0) den = L;
+        const float M = wave_max_v(mine.x, d), f = mine.y != 0.0f ? mine.y * __builtin_amdgcn_exp2f(mine.x - M) : 0.0f;
+        const float L = wave_sum_v(f, d);
+        wt[d] = mine.y != 0.0f ? f / L : -1.0f;
     }
     __syncthreads();
     float o = 0.0f;
@@ -1111,7 +1115,7 @@ QP_DEV void attn_mx8_comb(const QpAttnArgs& a) {
         if (y) return;
         o = (o + sum[1][d]) + (sum[2][d] + sum[3][d]);
     }
-    gstore<float>(a.o + 4 * (row * a.hd + d), den == 0.0f ? 0.0f : o / den);
+    gstore<float>(a.o + 4 * (row * a.hd + d), o);
 }
 KERNEL __launch_bounds__(128) void qp_attn_mx8_comb(QpAttnArgs a) { attn_mx8_comb<1>(a); }
 KERNEL __launch_bounds__(512) void qp_attn_mx8_comb4(QpAttnArgs a) { attn_mx8_comb<4>(a); }

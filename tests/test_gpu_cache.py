@@ -691,3 +691,20 @@ def test_argmax_of_rows(quipu, dev, rows, n):
     quipu.dispatch("argmax", [("u", n), ("u", rows)], [0, dev.buf(v), out])
     got = dev.get(out, (rows + 1,), np.uint32)
     assert got[:rows].tolist() == [n // 2] * rows and got[rows] == 77
+
+
+@pytest.mark.parametrize("T,n,nh,nkv", [(1, 90, 4, 1), (1, 3000, 8, 2), (24, 900, 8, 2), (260, 5600, 32, 8)])
+def test_values_near_the_largest(quipu, dev, T, n, nh, nkv):
+    """Values up to 2^127: sums of probabilities times values leave f32's range, the outputs do not."""
+    hd = 128
+    rng = np.random.default_rng(22)
+    q = rng.standard_normal((T, nh, hd)).astype(np.float32)
+    k, v = rng.standard_normal((n, nkv, hd)), rng.uniform(0.5, 1, (n, nkv, hd)) * 2.0 ** 127
+    k[::7] *= 3
+    kc, vc, kh, vh = mx8.cache(MX8, k, v)
+    some = sampled(rng, T)
+    see = causal(T, n - T, 0, n)[some]
+    for ns in (0, 1):
+        got, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, MX8, n, ns=ns)
+        assert np.isfinite(got).all()
+        assert np.all(np.abs(got[some] - mx8.attend(q[some], kh, vh, see, scale)) <= bound(q[some], kh, vh, see, scale))
