@@ -68,11 +68,13 @@ QP_DEV void sincos_far(float x, float& sn_out, float& cs_out) {
     cs_out = q == 1 || q == 2 ? -b : b;
 }
 
-// 1 / sqrt(y) for y >= 0 (off by one step at most; the instruction takes no subnormal y)
+// 1 / sqrt(y) for y >= 0: the instruction (off by a step, and no subnormal y) and a step of Newton's, since a value next to the
+// border of two bytes of a block may fall to either side for any error
 QP_DEV float rsqrt_any(float y) {
     const bool tiny = y < 0x1p-100f;
-    const float r = __builtin_amdgcn_rsqf(tiny ? y * 0x1p100f : y);
-    return tiny ? r * 0x1p50f : r;
+    const float z = tiny ? y * 0x1p100f : y, r = __builtin_amdgcn_rsqf(z), n = fmaf(0.5f * r, fmaf(-z * r, r, 1.0f), r);
+    const float s = z > 0.0f && z < __builtin_inff() ? n : r;
+    return tiny ? s * 0x1p50f : s;
 }
 
 // A wavefront has one token (hd = 128) or two (hd = 64) of N heads of q, of k or of v, which share the token's angles; grid
