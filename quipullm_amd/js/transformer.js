@@ -600,12 +600,13 @@ class ModeloTransformer {
     if (this.arbol) return this.arbol;
     const gpu = this.gpu, TB = this.maxArbol, B = (n, l) => { const b = gpu.buffer(n, undefined, l); this.bufs.push(b); return b; };
     const a = { mask: B(4 * TB * Math.ceil(TB / 32), 'tree_mask'), pos: B(4 * TB, 'tree_pos'), idx: B(4 * TB, 'tree_path'),
+      maskSwa: this.ventana ? B(4 * TB * Math.ceil(TB / 32), 'tree_mask_swa') : null,
       logits: B(4 * TB * this.vocab, 'tree_logits'), sig: B(4 * TB, 'tree_next') };
     a.capas = this.capas.map((c) => ({
       guardar: this._guardar(c, a.pos),
       att: gpu.grupo('atencion_arbol', [gpu.uniforme([['u', this.hd], ['u', this.nh], ['u', this.nkv], ['u', c.swa],
         ['f', this.escAtt], ['u', c.anillo], ['u', this.fmtKV], ['u', c.slots], ['u', 0]]), this.bPaso, this.q, c.kc, c.vc, this.att,
-        a.mask, a.pos, null]),
+        c.swa ? a.maskSwa : a.mask, a.pos, null]),
     }));
     a.norma = gpu.grupo('rmsnorm', [gpu.uniforme([['u', this.D], ['u', 0], ['f', this.eps], ['u', 0]]), this.bPaso, this.x,
       this.normFinal, this.xn]);
@@ -623,19 +624,22 @@ class ModeloTransformer {
     if (padres.length !== T) throw new Error('one parent for each token of the tree');
     if (this.pos + T > this.ctx) throw new Error('context exceeded (' + this.ctx + ' tokens)');
     for (const id of ids) if (!(id >= 0 && id < this.vocab)) throw new Error('token id ' + id + ' outside the vocabulary');
-    const mask = new Uint32Array(T * W), pos = new Uint32Array(T);
+    // maskSwa: of a token's path, what the windowed layers' windows hold (the op's window is of the keys before the tree)
+    const mask = new Uint32Array(T * W), maskSwa = this.ventana ? new Uint32Array(T * W) : null, pos = new Uint32Array(T);
     for (let i = 0; i < T; i++) {
       const p = padres[i];
       if (!Number.isInteger(p) || p < -1 || p >= i) throw new Error('token ' + i + ' of the tree follows token ' + p);
       if (p >= 0) for (let w = 0; w < W; w++) mask[i * W + w] = mask[p * W + w];
       mask[i * W + (i >> 5)] |= 1 << (i & 31);
       pos[i] = p < 0 ? this.pos : pos[p] + 1;
+      if (maskSwa) for (let j = i, n = this.ventana; j >= 0 && n > 0; j = padres[j], n--) maskSwa[i * W + (j >> 5)] |= 1 << (j & 31);
     }
     const a = this._armarArbol();
     this.rama = null;
     gpu.escribir(this.bPaso, 0, new Uint32Array([T, this.pos, 0, 0]));
     gpu.escribir(this.bIds, 0, new Uint32Array(ids));
     gpu.escribir(a.mask, 0, mask);
+    if (maskSwa) gpu.escribir(a.maskSwa, 0, maskSwa);
     gpu.escribir(a.pos, 0, pos);
     const mm = this._despacharCapas(T, a);
     despachar(null, a.norma, T);

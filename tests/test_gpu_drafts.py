@@ -256,3 +256,76 @@ def test_rings_remember_what_was_overwritten(models_dir):
     assert r["b"] == 45 and r["c"] == 0 and r["d"] == 0
     assert r["cids"] == r["dids"] == r["want"]
     assert r["despues"] == 58 and r["antes"] < 56
+
+
+DEEP = r"""
+const fs = require('fs');
+const engine = require(%(eng)s);
+(async () => {
+  const m = await engine.cargarModelo(%(path)s, {ctx: 256, options: {kv_f16: %(kv)s === 'f16', kv_mx8: %(kv)s === 'mx8', batch: 32}});
+  const fd = fs.openSync(%(out)s, 'w'), escribe = (f) => fs.writeSync(fd, Buffer.from(f.buffer, f.byteOffset, f.byteLength));
+  await engine.prefill(m, %(prompt)s);
+  const sig = Array.from(m.verificarArbol(%(ids)s, %(padres)s, {logits: (i, f) => escribe(f)}));
+  m.aceptarRama(%(camino)s);
+  for (const t of %(despues)s) escribe(await m.forward([t], true));
+  fs.closeSync(fd);
+  m.volcarKV(%(kvf)s);
+  console.log(JSON.stringify({sig: sig, pos: m.pos, ventana: m.ventana}));
+  m.free();
+})().catch((e) => { console.error(e.stack); process.exit(1); });
+"""
+
+
+@pytest.mark.parametrize("kv,plen", [("f32", 38), ("f32", 20), ("f16", 20), ("mx8", 20)])
+@pytest.mark.parametrize("fork", [False, True])
+def test_trees_deeper_than_the_window(oracle, models_dir, tmp_path, kv, plen, fork):
+    """Trees of 32 tokens on windows of 24: a chain, and one of 29 that forks behind its 26th token.  A token sees of its
+    ancestors what one-token decoding sees: logits within 1e-3 relative of the oracle's, along the path and behind it (f32: along
+    both forks, the ring of 56 slots wrapping; f16 and 8 bits: given the cache's values)."""
+    name = "mini_gemma3_q4km_c"
+    path = synth.ensure_model(name, models_dir)
+    c = synth.CONFIGS[name]
+    prompt = [int(t) for t in synth.random_prompt(c.vocab, plen, 4)]
+    ids = [int(t) for t in synth.random_prompt(c.vocab, 32, 51)]
+    padres = [i - 1 for i in range(29)] + ([25, 29, 30] if fork else [28, 29, 30])
+    camino = [i for i in range(32) if not fork or i < 26 or i >= 29]
+    despues = [int(t) for t in synth.random_prompt(c.vocab, 3, 6)]
+    out, kvf = str(tmp_path / "lg.f32"), str(tmp_path / "kv.bin")
+    print("node deep tree", kv, plen, fork, flush=True)
+    script = DEEP % {k: json.dumps(x) for k, x in dict(eng=ENG, path=path, kv=kv, prompt=prompt, ids=ids, padres=padres,
+                                                       camino=camino, despues=despues, out=out, kvf=kvf).items()}
+    rc, o, err = run(["timeout", "-k", "5", "110", "node", "-e", script], timeout=120)
+    assert rc == 0, err[-3000:]
+    r = json.loads(o.strip().splitlines()[-1])
+    taken = plen + len(camino) + len(despues)
+    assert r["ventana"] == 24 and r["pos"] == taken
+    lg = np.fromfile(out, np.float32).reshape(-1, c.vocab)
+    assert r["sig"] == [int(np.argmax(f)) for f in lg[:32]]
+    m = oracle.Model(path, ctx=256, kv_f16=kv != "f32")
+    if kv != "f32":
+        ks, vs, _ = held_rows(kvf, c, slots_of(c, 256, 32), taken, mx8.MX8 if kv == "mx8" else mx8.F16)
+        m.set_kv_reference(*as_reference(ks, vs))
+    errs = {}
+    for way in [list(range(29)), camino] if fork and kv == "f32" else [camino]:
+        m.reset()
+        m.forward(prompt[:32], False)
+        if plen > 32:
+            m.forward(prompt[32:], False)
+        for i in way:
+            errs[i] = rel(lg[i], m.forward([ids[i]]))
+    for k, t in enumerate(despues):
+        errs["after %d" % k] = rel(lg[32 + k], m.forward([t]))
+    m.close()
+    print({k: float("%.2g" % x) for k, x in errs.items()}, flush=True)
+    assert max(errs.values()) < 1e-3, errs
+
+
+@pytest.mark.parametrize("kv", ["f32", "mx8"])
+def test_looked_up_drafts_deeper_than_the_window(models_dir, tmp_path, kv):
+    """As test_looked_up_drafts_give_the_greedy_ids, with chains of 31 drafted tokens on windows of 24."""
+    path = synth.ensure_model("mini_gemma3_q4km_c", models_dir)
+    prompt = [int(t) for t in synth.random_prompt(1000, 40, 31)] * 2
+    a, _ = generate(path, prompt, 60, "engine", kv, str(tmp_path))
+    b, _ = generate(path, prompt, 60, "engine", kv, str(tmp_path), ["--drafts", "31"])
+    print(kv, b["drafts"], flush=True)
+    assert a["ids"] == b["ids"]
