@@ -461,21 +461,25 @@ struct MxState {
             for (int d = 0; d < DT; d++) o[r][d] = f32x4{0, 0, 0, 0};
         }
     }
-    // Accumulators s of the lane's 8 keys of each row (scores: times unit, in units of log2): those of keys that the row does not
-    // see become -inf, and the row's reference m follows them.  c: what s is to be multiplied by from now on.
+    // Accumulators s of the lane's 8 keys of each row: those of keys that the row does not see become -inf.
+    template <class W>
+    QP_DEV void hide(const W& w, const typename W::Tile& t, f32x4 (&s)[RG][2]) const {
+        if (w.all_see(t, w.t_lo, w.t_hi)) return;
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            const uint32_t bits = w.drafted(t, r);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                s[r][j >> 2][j & 3] = w.sees(t, r, (j >> 2) * 16 + 4 * w.g + (j & 3), bits) ? s[r][j >> 2][j & 3] : -__builtin_inff();
+        }
+    }
+    // The same, and the row's reference m follows them (scores: s times unit, in units of log2).  c: what s is to be multiplied by
+    // from now on.
     template <class W>
     QP_DEV void follow(const W& w, const typename W::Tile& t, f32x4 (&s)[RG][2], const float (&unit)[RG], float (&c)[RG]) {
 #pragma unroll
         for (int r = 0; r < RG; r++) c[r] = unit[r];
-        if (!w.all_see(t, w.t_lo, w.t_hi)) {
-#pragma unroll
-            for (int r = 0; r < RG; r++) {
-                const uint32_t bits = w.drafted(t, r);
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    s[r][j >> 2][j & 3] = w.sees(t, r, (j >> 2) * 16 + 4 * w.g + (j & 3), bits) ? s[r][j >> 2][j & 3] : -__builtin_inff();
-            }
-        }
+        hide(w, t, s);
         float mx[RG];
         bool past = false;
 #pragma unroll
@@ -552,14 +556,50 @@ struct MxState {
             l[r] += bfly_f<5>(l[r], lane);
         }
     }
+    // The same for a state that holds its outputs over their sums, with the largest scores themselves as references: o becomes
+    // o (l 2^(m - m')) / l' and p 2^(s - m') / l', so that o stays within the values whatever they are.  l: the row's, not the
+    // lane's.  (No key seen: l = 0, o = 0.)
+    template <class W>
+    QP_DEV void follow_over(const W& w, const typename W::Tile& t, f32x4 (&s)[RG][2], float c) {
+#pragma clang fp contract(off)  // (s c - m in one rounding could be as large as half of m's last place)
+        hide(w, t, s);
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                s[r][j >> 2][j & 3] *= c;
+                top = fmaxf(top, s[r][j >> 2][j & 3]);
+            }
+            top = fmaxf(top, bfly_f<4>(top, w.lane));
+            top = fmaxf(top, bfly_f<5>(top, w.lane));
+            const float mn = fmaxf(m[r], top), was = l[r] * __builtin_amdgcn_exp2f(m[r] - mn);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                p[r][j] = __builtin_amdgcn_exp2f(s[r][j >> 2][j & 3] - mn);
+                sum += p[r][j];
+            }
+            sum += bfly_f<4>(sum, w.lane);
+            sum += bfly_f<5>(sum, w.lane);
+            m[r] = mn;
+            l[r] = was + sum;
+            const float n = l[r] == 0.0f ? 0.0f : 1.0f / l[r], f = was * n;
+#pragma unroll
+            for (int j = 0; j < 8; j++) p[r][j] *= n;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[r][d][x] *= f;
+        }
+    }
     // channels DT (4 g + x) + d .. d + 3, times 2^back, over l (no key seen: l = 0, o = 0)
     QP_DEV float4 out4(int r, int x, int d, int back) const {
         const float f = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
         return make_float4(__builtin_ldexpf(o[r][d][x] * f, back), __builtin_ldexpf(o[r][d + 1][x] * f, back),
                            __builtin_ldexpf(o[r][d + 2][x] * f, back), __builtin_ldexpf(o[r][d + 3][x] * f, back));
     }
-    template <class W>
-    QP_DEV void put_all(const W& w, int back) const {
+    template <bool OVER, class W>
+    QP_DEV void put_all(const W& w, int back) const {  // OVER: o is over l already
 #pragma unroll
         for (int r = 0; r < RG; r++) {
             const uint32_t row = w.r0 + r * 16 + w.n16;
@@ -567,12 +607,15 @@ struct MxState {
 #pragma unroll
             for (int x = 0; x < 4; x++)
 #pragma unroll
-                for (int d = 0; d < DT; d += 4) w.put(row, DT * (4 * w.g + x) + d, out4(r, x, d, back), m[r], l[r]);
+                for (int d = 0; d < DT; d += 4)
+                    w.put(row, DT * (4 * w.g + x) + d,
+                          OVER ? make_float4(o[r][d][x], o[r][d + 1][x], o[r][d + 2][x], o[r][d + 3][x]) : out4(r, x, d, back), m[r], l[r]);
         }
     }
 };
 
-// The workgroup's rows in f32, its share of the keys from the first tile on.  Not WIDE: by the first wavefront alone.
+// The workgroup's rows in f32, its share of the keys from the first tile on.  Not WIDE: by the first wavefront alone.  Values come
+// as they are, up to f32's largest and beside small ones: no power of two below them all, so outputs are held over their sums.
 template <int HD, int RG, bool TREE, bool WIDE>
 __device__ __attribute__((noinline)) void attn_mx8_f32(const __attribute__((address_space(4))) QpAttnArgs* args) {
     const QpAttnArgs a = *args;
@@ -582,9 +625,6 @@ __device__ __attribute__((noinline)) void attn_mx8_f32(const __attribute__((addr
     MxState<HD, RG> st;
     st.start();
     const float scale = a.scale * MX_LOG2E, sign = scale < 0.0f ? -1.0f : 1.0f;
-    float c[RG];
-#pragma unroll
-    for (int r = 0; r < RG; r++) c[r] = fmaxf(fabsf(scale), 1.2e-38f);
     const uint64_t kb = a.kc + w.hk + w.lane * 16, vb = a.vc + w.hk + w.lane * 16, kx = a.kc + w.hx, vx = a.vc + w.hx;
     for (uint32_t i = w.i0; i < w.i1; i++) {
         const typename W::Tile t = w.tile(i);
@@ -604,9 +644,7 @@ __device__ __attribute__((noinline)) void attn_mx8_f32(const __attribute__((addr
                     for (int r = 0; r < RG; r++)
                         s[r][h] = mx_mfma(mx_value((k[b >> 2] >> (8 * (b & 3))) & 255, x), gload<float>(w.query(r) + cc * 256 + 4 * b) * sign, s[r][h]);
             }
-        float d[RG];
-        st.follow(w, t, s, c, d);
-        st.weigh(s, d);
+        st.follow_over(w, t, s, fmaxf(fabsf(scale), 1.2e-38f));
         const bool whole = w.all_see(t, w.t_lo, w.t_hi);
         uint32_t x[8];
         bool bad = false;
@@ -628,8 +666,7 @@ __device__ __attribute__((noinline)) void attn_mx8_f32(const __attribute__((addr
                     st.o[r][d] = mx_mfma(mx_value(((j < 4 ? v.x : v.y) >> (8 * (j & 3))) & 255, x[j]), st.p[r][j], st.o[r][d]);
         }
     }
-    st.sum_l(w.lane);
-    st.put_all(w, 0);
+    st.template put_all<true>(w, 0);
 }
 
 template <int HD, int RG, bool TREE, bool WIDE>
@@ -1027,7 +1064,7 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     const int back = ev - 138;  // o times 2^back: the outputs
     st.sum_l(lane);
     if constexpr (WIDE) {
-        st.put_all(w, back);
+        st.template put_all<false>(w, back);
     } else {
         // ---- the four wavefronts' states meet: [wave][row][HD + 4], then [wave][row] (m, l)
         constexpr int LD = HD + 4;
