@@ -561,15 +561,16 @@ struct MxState {
     // lane's.  (No key seen: l = 0, o = 0.)
     template <class W>
     QP_DEV void follow_over(const W& w, const typename W::Tile& t, f32x4 (&s)[RG][2], float c) {
-#pragma clang fp contract(off)  // (s c - m in one rounding could be as large as half of m's last place)
         hide(w, t, s);
 #pragma unroll
         for (int r = 0; r < RG; r++) {
             float top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                s[r][j >> 2][j & 3] *= c;
-                top = fmaxf(top, s[r][j >> 2][j & 3]);
+                float v = s[r][j >> 2][j & 3] * c;
+                asm("" : "+v"(v));  // (s c - m in one rounding could be as large as half of m's last place)
+                s[r][j >> 2][j & 3] = v;
+                top = fmaxf(top, v);
             }
             top = fmaxf(top, bfly_f<4>(top, w.lane));
             top = fmaxf(top, bfly_f<5>(top, w.lane));
@@ -773,7 +774,7 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     MxState<HD, RG> st;
     st.start();
     int ek = 20, ev = 20;  // E of the keys and values (20 at least)
-    bool any_v = false;    // ev has been set
+    int ev_span = -1;      // the lowest and (<< 8) the highest that ev has been since it was set; -1: it has not been
     int moved = 0;         // the sums are to be multiplied by 2^moved (ev has changed)
     float cs[RG];          // score = accumulator times cs, in units of log2, of keys unpacked with E = ek
     auto unit = [&](int e, float (&c)[RG]) __attribute__((always_inline)) {
@@ -832,10 +833,12 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
             x = range_v();
         }
         const int e = settle(x.lo, x.hi, ev);
-        moved = any_v ? ev - e : 0;
-        any_v = any_v || __any(x.hi != 0);
+        const bool set = ev_span >= 0;
+        const int lo = set ? min(ev_span & 255, e) : e, hi = set ? max(ev_span >> 8, e) : e;
+        moved = set ? ev - e : 0;
+        if (__any(x.hi != 0)) ev_span = lo | (hi << 8);
         ev = e;
-        return e < 256 && abs(moved) <= 60;  // (the sums could leave f32's range)
+        return e < 256 && hi - lo <= 60;  // (the sums, moved by all steps together, could leave f32's range)
     };
     auto move = [&]() __attribute__((always_inline)) {
         if (moved == 0) return;

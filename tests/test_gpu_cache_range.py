@@ -68,3 +68,28 @@ def test_values_near_the_largest_in_f32(quipu, dev, T, n, nh, nkv, hd, kind, tre
     for ns in (0, 1, 5):
         got, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, MX8, n, ns=ns, mask=chain(T) if tree else None)
         check(got, q, kh, vh, see, scale, sampled(rng, T))
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", ["falling", "rising_without_weight"])
+@pytest.mark.parametrize("T,n,nh,nkv,run", [(24, 1700, 8, 2, 512), (1, 1300, 4, 1, 384), (1040, 1500, 32, 8, 128), (1, 100000, 4, 2, 8192)])
+def test_values_that_move_the_scale_again_and_again(quipu, dev, T, n, nh, nkv, run, kind, hd, tree):
+    """Values whose magnitudes fall by 2^54 three times along the keys, and ones that rise so from keys that alone have weight:
+    each step is one that the sums bear, all together are not."""
+    rng = np.random.default_rng(32)
+    q = rng.standard_normal((T, nh, hd)).astype(np.float32)
+    k, v = (rng.standard_normal((n, nkv, hd)) for _ in "kv")
+    level = np.minimum(np.arange(n) // run, 3)
+    if kind == "falling":
+        v *= 2.0 ** (100 - 54.0 * level)[:, None, None]
+    else:
+        v *= 2.0 ** (-100 + 54.0 * level)[:, None, None]
+        q[..., 0] = 4
+        k[:, :, 0] = np.where(level > 0, -3000, 0)[:, None]
+        k[level > 0, :, 1:32] = 0
+    kc, vc, kh, vh = mx8.cache(MX8, k, v)
+    see = causal(T, n - T, 0, n)
+    for ns in (1, 0):
+        got, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, MX8, n, ns=ns, mask=chain(T) if tree else None)
+        check(got, q, kh, vh, see, scale, sampled(rng, T))
