@@ -57,6 +57,10 @@ typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 template <int HD, bool F16, int RG, bool TREE = false>
 QP_DEV void attn_x_body(const QpAttnArgs& a) {
     constexpr int KS = HD / 32, DT = HD / 16;  // steps of 32 dimensions, tiles of 16 (DT dimensions per lane of 16)
+    // trees over f32 caches: outputs are held over their sums wherever values come as they are (f32 tiles, the meetings of
+    // states), so that they stay within the values, up to f32's largest (8 tokens behind 4100 keys of 8 heads 22.0 us, 21.5 with
+    // the sums beside them; 64 behind 32000 of 4 274, 273)
+    constexpr bool OVER = TREE && !F16;
     extern __shared__ float4 ax_lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n16 = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -296,6 +300,23 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
 #pragma unroll
                 for (int x = 0; x < 4; x++) o[r][d][x] *= corr[r] * f;
     };
+    // OVER, f32 tiles: the row's sum so far over all its lanes; o times before, p and what o was over give way to it
+    float lrow[RG];
+    auto divide = [&](bool had, float back) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < RG; r++) {
+            float sum = l[r] + bfly_f<4>(l[r], lane);
+            sum += bfly_f<5>(sum, lane);
+            const float n = sum == 0.0f ? 0.0f : 1.0f / sum, f = had ? lrow[r] * corr[r] * n : corr[r] * n;
+            lrow[r] = sum;
+#pragma unroll
+            for (int j = 0; j < 8; j++) p[r][j] *= n;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[r][d][x] = (o[r][d][x] * f) * back;
+        }
+    };
     auto pv_f32 = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -423,12 +444,14 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
         load_v(i + 4);
     }
     float back = (F16 ? 1.0f : ax_pow2(ev - 9)) * 0x1p-10f;  // o times it: the outputs
+    const bool in_f32 = i < i1;
     if (i < i1) {  // the other tiles in f32
         if (!pending) {
 #pragma unroll
             for (int r = 0; r < RG; r++) corr[r] = 1.0f;
         }
-        rescale(back);
+        if constexpr (OVER) divide(false, back);
+        else rescale(back);
         back = 1.0f;
         if (pending) {
             pv_f32();
@@ -457,7 +480,8 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
             softmax(t, s, SkInt<0>(), a.scale * AX_LOG2E);
             mask_v(t);
             if constexpr (TREE) poison(t);
-            rescale(1.0f);
+            if constexpr (OVER) divide(true, 1.0f);
+            else rescale(1.0f);
             pv_f32();
             load_v(i + 4);
         }
@@ -472,6 +496,7 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
         lt += bfly_f<4>(lt, lane);
         lt += bfly_f<5>(lt, lane);
         const uint32_t at = wave * RG * 16 + r * 16 + n16;
+        const float over = !OVER || in_f32 ? 1.0f : lt == 0.0f ? 0.0f : 1.0f / lt;
         if (g == 0) {
             ml[2 * at] = m[r];
             ml[2 * at + 1] = lt;
@@ -482,7 +507,8 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
 #pragma unroll
             for (int d = 0; d < DT; d += 4)
                 *reinterpret_cast<float4*>(ol + at * LD + DT * (4 * g + x) + d) =
-                    make_float4(o[r][d][x] * back, o[r][d + 1][x] * back, o[r][d + 2][x] * back, o[r][d + 3][x] * back);
+                    make_float4(o[r][d][x] * over * back, o[r][d + 1][x] * over * back, o[r][d + 2][x] * over * back,
+                                o[r][d + 3][x] * over * back);
     }
     __syncthreads();
     for (uint32_t k = tid; k < RG * 16 * (HD / 4); k += 256) {
@@ -491,25 +517,34 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
         float M = -3.0e38f;
 #pragma unroll
         for (int w = 0; w < 4; w++) M = fmaxf(M, ml[2 * (w * RG * 16 + lr)]);
-        float L = 0.0f;
+        float L = 0.0f, n = 0.0f;
         float4 s = make_float4(0, 0, 0, 0);
+        if constexpr (OVER) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const uint32_t at = w * RG * 16 + lr;
+                L += ml[2 * at + 1] != 0.0f ? ml[2 * at + 1] * __builtin_amdgcn_exp2f(ml[2 * at] - M) : 0.0f;
+            }
+            n = L == 0.0f ? 0.0f : 1.0f / L;
+        }
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const uint32_t at = w * RG * 16 + lr;
-            const float lw = ml[2 * at + 1], f = lw != 0.0f ? __builtin_amdgcn_exp2f(ml[2 * at] - M) : 0.0f;
+            const float lw = ml[2 * at + 1], e = lw != 0.0f ? __builtin_amdgcn_exp2f(ml[2 * at] - M) : 0.0f, f = OVER ? lw * e * n : e;
             const float4 v = *reinterpret_cast<const float4*>(ol + at * LD + 4 * c);
-            L += lw * f;
+            if constexpr (!OVER) L += lw * f;
             if (TREE ? lw != 0.0f : f != 0.0f) s = make_float4(s.x + v.x * f, s.y + v.y * f, s.z + v.z * f, s.w + v.w * f);
         }
         const uint32_t t = row / G, h = kvh * G + row % G;
         const uint64_t at = (uint64_t)t * a.nh + h;
         if (a.nsplit == 1) {
             const bool none = TREE && L == 0.0f;
-            gstore<float4>(a.o + 4 * (at * HD + 4 * c), none ? make_float4(0, 0, 0, 0) : make_float4(s.x / L, s.y / L, s.z / L, s.w / L));
+            if constexpr (!OVER) s = none ? make_float4(0, 0, 0, 0) : make_float4(s.x / L, s.y / L, s.z / L, s.w / L);
+            gstore<float4>(a.o + 4 * (at * HD + 4 * c), s);
         } else {
             // (TREE: met by qp_attn_mx8_comb, which takes outputs)
-            const float n = !TREE ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
-            gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + 4 * c), make_float4(s.x * n, s.y * n, s.z * n, s.w * n));
+            const float over = TREE && !OVER ? L == 0.0f ? 0.0f : 1.0f / L : 1.0f;
+            gstore<float4>(a.part_o + 4 * ((at * a.nsplit + blockIdx.z) * HD + 4 * c), make_float4(s.x * over, s.y * over, s.z * over, s.w * over));
             if (c == 0) gstore<float2>(a.part_ml + 8 * (at * a.nsplit + blockIdx.z), make_float2(M, L));
         }
     }

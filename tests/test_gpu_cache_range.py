@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 import mx8
-from mx8 import MX8
+from mx8 import F32, MX8
 from test_gpu_cache import causal, run_attention, sampled
 from test_gpu_ops import dev  # noqa: F401
 
@@ -92,4 +92,26 @@ def test_values_that_move_the_scale_again_and_again(quipu, dev, T, n, nh, nkv, r
     see = causal(T, n - T, 0, n)
     for ns in (1, 0):
         got, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, MX8, n, ns=ns, mask=chain(T) if tree else None)
+        check(got, q, kh, vh, see, scale, sampled(rng, T))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("T,n,nh,nkv", [(1, 3, 1, 1), (1, 90, 4, 1), (24, 900, 8, 2), (100, 4000, 16, 8)])
+@pytest.mark.parametrize("kind", ["alike", "beside_ones", "nan_key"])
+@pytest.mark.parametrize("fmt", [F32, MX8])
+def test_tree_values_near_the_largest(quipu, dev, fmt, T, n, nh, nkv, kind, hd):
+    """atencion_arbol over values up to 2^127: sums of probabilities times values leave float32's range, the outputs do not."""
+    rng = np.random.default_rng(33)
+    q = rng.standard_normal((T, nh, hd)).astype(np.float32)
+    k, v = rng.standard_normal((n, nkv, hd)), rng.uniform(0.5, 1, (n, nkv, hd)) * 2.0 ** 127
+    if n == 3:
+        k[:] = 0
+    if kind == "beside_ones":
+        v[1::2] = rng.standard_normal((len(v[1::2]), nkv, hd))
+    elif kind == "nan_key" and T > 1:
+        k[n - T // 2, :, 5] = np.nan
+    kc, vc, kh, vh = mx8.cache(fmt, k, v)
+    see = causal(T, n - T, 0, n)
+    for ns in (0, 1, 5):
+        got, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, fmt, n, ns=ns, mask=chain(T))
         check(got, q, kh, vh, see, scale, sampled(rng, T))
