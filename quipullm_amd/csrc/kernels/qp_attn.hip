@@ -207,7 +207,10 @@ QP_DEV void attn_x_body(const QpAttnArgs& a) {
         const bool whole = all_see(t);
 #pragma unroll
         for (int r = 0; r < RG; r++) {
-            const float c = Split.v ? qs[r] * unit : unit;
+            float c = Split.v ? qs[r] * unit : unit;
+            // (accumulators are multiples of 2^-48 below 2^34: from 2^88 on two that differ are a weight of 0 apart, and no score
+            // leaves f32's range)
+            if constexpr (TREE && Split.v) c = __builtin_amdgcn_fmed3f(c, -0x1p88f, 0x1p88f);
             uint32_t bits = 0;
             if constexpr (TREE) bits = whole ? 0 : drafted(t, r);
             float x[8], mx = -3.0e38f;

@@ -777,9 +777,11 @@ QP_DEV void attn_mx8_body(const QpAttnArgs& a) {
     int ev_span = -1;      // the lowest and (<< 8) the highest that ev has been since it was set; -1: it has not been
     int moved = 0;         // the sums are to be multiplied by 2^moved (ev has changed)
     float cs[RG];          // score = accumulator times cs, in units of log2, of keys unpacked with E = ek
+    // (at most 2^88: accumulators are multiples of 2^-38 below 2^34, so that from there on two that differ are a weight of 0 apart,
+    // and no score leaves f32's range)
     auto unit = [&](int e, float (&c)[RG]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int r = 0; r < RG; r++) c[r] = fmaxf(__builtin_ldexpf(scale, e + qe[r] - 152), 1.2e-38f);
+        for (int r = 0; r < RG; r++) c[r] = __builtin_amdgcn_fmed3f(__builtin_ldexpf(scale, e + qe[r] - 152), 1.2e-38f, 0x1p88f);
     };
     auto wave_most = [&](int x) __attribute__((always_inline)) {  // of whole numbers below 2^24
         return (int)__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max_v((float)x, lane))));

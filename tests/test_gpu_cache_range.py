@@ -115,3 +115,25 @@ def test_tree_values_near_the_largest(quipu, dev, fmt, T, n, nh, nkv, kind, hd):
     for ns in (0, 1, 5):
         got, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, fmt, n, ns=ns, mask=chain(T))
         check(got, q, kh, vh, see, scale, sampled(rng, T))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("T,n,nh,nkv", [(24, 90, 8, 2), (1, 500, 4, 1), (1040, 1100, 32, 8)])
+@pytest.mark.parametrize("op,fmt", [("mx8", MX8), ("tree", MX8), ("tree", F32)])
+def test_magnitudes_whose_product_float32_does_not_hold(quipu, dev, op, fmt, T, n, nh, nkv, hd):
+    """Queries of 2^40 in channels where the keys are 0, keys of 2^121 in channels where the queries are 0: scores of 0.  And
+    one key with a score of 2^40."""
+    rng = np.random.default_rng(34)
+    q, k, v = np.zeros((T, nh, hd), np.float32), np.zeros((n, nkv, hd)), rng.standard_normal((n, nkv, hd))
+    q[..., 0:hd:32], k[..., 1:hd:32] = 2.0 ** 40, 2.0 ** 121
+    if fmt == MX8:
+        k[..., 0:32] = 0
+        q[..., 32:] = 0
+    if T == 1:
+        k[n // 2] = 0
+        k[n // 2, :, 0] = 1
+    kc, vc, kh, vh = mx8.cache(fmt, k, v)
+    see = causal(T, n - T, 0, n)
+    for ns in (0, 1, 5):
+        got, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, fmt, n, ns=ns, mask=chain(T) if op == "tree" else None)
+        check(got, q, kh, vh, see, scale, sampled(rng, T))
