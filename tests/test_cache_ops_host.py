@@ -223,3 +223,68 @@ def test_argmax_rows(lib):
     for u in ([100, 8], [101, 7], [1, 8], [1, 65536]):
         err, log = lib.dispatch("argmax", u, [0, v, out], (1,))
         assert "argmax" in err and not log
+
+
+def exact_calls():
+    """(op, fmt, T, hd, given shares): each operator with every cache type and head size, a mask of one word a row and of two."""
+    for op in OPS:
+        for fmt in (0, 1, 2):
+            if op == "atencion_mx8" and fmt != 2:
+                continue
+            for T, hd in ((5, 128), (33, 64)):
+                yield op, fmt, T, hd, 0
+                if op.startswith("atencion"):
+                    yield op, fmt, T, hd, 3
+
+
+@pytest.mark.parametrize("op,fmt,T,hd,ns", list(exact_calls()))
+def test_bindings_of_exactly_what_is_needed(lib, op, fmt, T, hd, ns):
+    """Buffers of exactly the bytes that the call reads or writes are taken; each binding one element (4 bytes) further on is
+    refused, by a message that names it."""
+    nh, nkv, rows = 8, 2, 101
+    c = Call(lib, op, fmt, T=T, hd=hd, nh=nh, nkv=nkv, rows=rows, swa=40 if op.startswith("atencion") else 0)
+    r32 = 128
+    k = v = 4 * rows * nkv * hd
+    if fmt == 1:
+        k, v = 2 * rows * nkv * hd, 2 * r32 * nkv * hd
+    elif fmt == 2:
+        k = v = r32 * nkv * (hd + hd // 32)
+    heads = lambda h: 4 * T * h * hd   # noqa: E731
+    need = {"kc": (k, "the K cache"), "vc": (v, "the V cache")}
+    if op == "norm_rope_kv":
+        need.update(q=(heads(nh), "q"), qo=(heads(nh), "the output of q"), k=(heads(nkv), "k"), v=(heads(nkv), "v"),
+                    qnorm=(4 * hd, "q's norm"), knorm=(4 * hd, "k's norm"), freq=(4 * (hd // 2), "the frequency table"),
+                    pos=(4 * T, "the positions"))
+    elif op == "kv_read":
+        need.update(k=(heads(nkv), "the keys' rows"), v=(heads(nkv), "the values' rows"))
+    elif op == "kv_ramal":
+        need.update(idx=(4 * T, "the path"))
+    else:
+        need.update(q=(heads(nh), "q"), o=(heads(nh), "the output"))
+        if op == "atencion_arbol":
+            need.update(mask=(4 * T * ((T + 31) // 32), "the mask"), pos=(4 * T, "the positions"))
+        if ns:
+            need.update(parts=(ns * T * nh * (4 * hd + 8), "the shares' buffer"))
+            c.u[c.names.index("ns")] = ns
+    assert set(need) == set(n for n, p in zip(c.bnames, c.b) if p or n == "parts" and ns) - {"paso"}
+    bufs = {n: lib.buf(size) for n, (size, _) in need.items()}
+    err, log = c.run(**bufs)
+    assert not err and log, err
+    for n, (size, what) in need.items():
+        err, log = c.run(**dict(bufs, **{n: bufs[n] + 4}))
+        assert err.startswith("%s: %s holds %d bytes" % (op, what, size - 4)) and not log, (n, err)
+
+
+def test_read_rows_of_16_bits_exactly(lib):
+    c = Call(lib, "kv_read", 1, T=5, hd=64, nkv=2)
+    k, v = (lib.buf(2 * 5 * 2 * 64) for _ in "kv")
+    assert not c.run(out=1, k=k, v=v)[0]
+    assert "the keys' rows holds" in c.run(out=1, k=k + 4, v=v)[0] and "the values' rows holds" in c.run(out=1, k=k, v=v + 4)[0]
+    assert "holds" in c.run(out=0, k=k, v=v)[0]
+
+
+def test_argmax_rows_exactly(lib):
+    v, out = lib.buf(4 * 100 * 7), lib.buf(4 * 7)
+    assert not lib.dispatch("argmax", [100, 7], [0, v, out], (1,))[0]
+    assert "the rows holds" in lib.dispatch("argmax", [100, 7], [0, v + 4, out], (1,))[0]
+    assert "the output holds" in lib.dispatch("argmax", [100, 7], [0, v, out + 4], (1,))[0]
