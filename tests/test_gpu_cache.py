@@ -708,3 +708,40 @@ def test_values_near_the_largest(quipu, dev, T, n, nh, nkv):
         got, scale = run_attention(quipu, dev, q, kc, vc, T, n - T, nkv, MX8, n, ns=ns)
         assert np.isfinite(got).all()
         assert np.all(np.abs(got[some] - mx8.attend(q[some], kh, vh, see, scale)) <= bound(q[some], kh, vh, see, scale))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,nh,nkv,T,pos0,nrot,neox,norm,cap", [
+    (128, 30, 7, 400, 11, 128, 0, 1, 0),      # groups of four with two and three heads in the last ones
+    (128, 30, 7, 403, 0, 128, 1, 1, 450),     # halves apart (through LDS), a ring
+    (64, 27, 5, 901, 5, 64, 1, 1, 0),         # two tokens for each wavefront, the last alone; three and one heads
+    (64, 27, 5, 950, 1000, 22, 0, 0, 951),
+    (128, 1, 31, 301, 3, 34, 1, 0, 0),        # one head of q
+    (64, 33, 16, 700, 77, 0, 0, 1, 0),        # norms alone
+])
+def test_stores_of_many_tokens(quipu, dev, fmt, hd, nh, nkv, T, pos0, nrot, neox, norm, cap):
+    """As test_rotation, with tokens enough that a wavefront takes four heads (64 wavefronts for each of 256 CUs); the rows
+    behind the Paso's tokens stay as they were."""
+    assert T * (nh + 2 * nkv) * hd // 128 >= 64 * 256
+    rng = np.random.default_rng(23)
+    q, k, v = (rng.standard_normal((T, h, hd)).astype(np.float32) for h in (nh, nkv, nkv))
+    qn, kn = ((1 + 0.2 * rng.standard_normal(hd)).astype(np.float32) for _ in "qk") if norm else (None, None)
+    rows = cap or pos0 + T + 3
+    n = T - 5  # the Paso's
+    qo, kc, vc, hs = store(quipu, dev, q, k, v, pos0, rows, fmt, cap, neox, nrot, qn, kn, T=n, fill=0)
+    pos = pos0 + np.arange(T)
+    want, size = rotate(q, qn, pos, nrot, neox)
+    assert np.all(np.abs(qo - want)[:n] <= ROT * size[:n]) and np.all(qo[n:] == 7.0)
+    gk, gv = (x.astype(np.float64) for x in read(quipu, dev, hs, nkv, hd, fmt, rows, pos0, n, cap))
+    want, size = (x[:n] for x in rotate(k, kn, pos, nrot, neox))
+    if fmt == F32:
+        assert np.all(np.abs(gk - want) <= ROT * size) and np.array_equal(gv, v[:n])
+    elif fmt == F16:
+        assert np.all(np.abs(gk - want) <= ROT * size + 2.0 ** -11 * np.abs(want) + 2.0 ** -25)
+        assert np.array_equal(gv, v[:n].astype(np.float16))
+    else:
+        step = 2.0 ** (mx8.quantise(want.astype(np.float32))[1].astype(np.float64) - 133).repeat(32, -1)
+        assert np.all(np.abs(gk - want) <= 0.5 * step + 2 * ROT * size + 0.5 * step * (np.abs(want) > 63 * step))
+        assert np.array_equal(gv, mx8.dequantise(*mx8.quantise(v[:n])))
+    inplace = store(quipu, dev, q, k, v, pos0, rows, fmt, cap, neox, nrot, qn, kn, T=n, inplace=True)[0]
+    assert np.array_equal(inplace[:n], qo[:n]) and np.array_equal(inplace[n:], q[n:])
