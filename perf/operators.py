@@ -10,6 +10,8 @@ A pass is one of
           read back with kv_read
 
 `own` chooses between the backend's ops and their plain form in torch operations.
+The ops run on the backend's own stream: the first pass over a state waits for what torch was asked for before, and a caller
+waits for the device before torch reads what a pass gave or changes what it reads.
 
 Cache layouts (R slots: the rows rounded up to 32; a tile is 32 slots).
   f32  K and V [slot][nkv hd]
@@ -395,6 +397,7 @@ def run(s):
     if own:
         if "plan" not in s:
             s["plan"] = plan(s)
+            torch.cuda.synchronize()   # the backend's stream does not wait for torch's: the inputs and the buffers are ready
         return s["plan"].run()
     return run_plain(s)
 
