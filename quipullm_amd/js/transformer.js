@@ -697,7 +697,7 @@ class ModeloTransformer {
   // is kept, with its own next choice.  Consumes `primero`, processes n ids and returns the n ids that follow them, as
   // decodificarVoraz does.  opciones.cuenta, if given, counts {pasos, aceptados}.
   decodificarRamas(primero, n, opciones) {
-    const op = opciones || {}, max = Math.min(this.maxArbol, 1 + (op.ramas || 16)), out = [], cuenta = op.cuenta || {};
+    const op = opciones || {}, max = Math.min(this.maxArbol, 1 + Math.floor(op.ramas || 16)), out = [], cuenta = op.cuenta || {};
     if (n < 1) return out;
     if (this.pos + n > this.ctx) throw new Error('context exceeded (' + this.ctx + ' tokens)');
     cuenta.pasos = cuenta.pasos || 0;
@@ -1110,6 +1110,7 @@ function tablaRope(base, nrot) {
 // the last 3, then 2, then 1 ids, the most recent first, at most max tokens in all and `largo` below the root.
 function arbolDe(h, max, largo) {
   const N = h.length, ids = [h[N - 1]], padres = [-1], hijos = [new Map()];
+  max = Math.floor(max);
   for (let g = Math.min(3, N - 1); g >= 1 && ids.length < max; g--) {
     for (let j = N - 2; j >= g - 1 && ids.length < max; j--) {
       let igual = true;

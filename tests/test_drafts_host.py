@@ -51,3 +51,13 @@ def test_limits(most, deep):
         while a["padres"][j] >= 0:
             d, j = d + 1, a["padres"][j]
         assert d <= deep - 1
+
+
+@pytest.mark.parametrize("most", [1.5, 2.5, 4.25])
+def test_limits_that_are_no_whole_numbers(most):
+    """A tree stays below the limit, whole or not."""
+    s = ("const {arbolDe} = require(%s); console.log(arbolDe(%s, %s, 9).ids.length);"
+         % (json.dumps(TF), json.dumps([1, 2, 3, 4, 5, 6, 7, 8, 9, 1, 2]), most))
+    out = subprocess.run(["node", "-e", s], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0, out.stderr
+    assert int(out.stdout) <= most
