@@ -318,10 +318,11 @@ constexpr float MX_LOG2E = 1.4426950408889634f;
 // Scores are S^T = K Q^T and outputs O^T += V^T P^T with v_mfma_f32_16x16x32_f16: a lane holds 8 scores of one row, which are its
 // operand of the second product.  Queries and probabilities are f16 high and low parts (22 bits) below a power of two.  Keys and
 // values are q 2^(x - E + 5) with an E of their own, exact and normal for x - E = -19 .. 0; a tile with blocks outside that
-// range moves E (and the sums so far with it).  Where no E will do (blocks of one tile further apart than 2^19, or not finite;
-// eight inputs of a query that are all below 2^-16 of its largest, whose parts would lose bits, or not finite), the workgroup
-// computes its rows with the f32 matrix instruction instead (attn_mx8_f32, some ten times slower).  So no row loses bits to a
-// key that it does not see.
+// range moves E (and the sums so far with it).  Where no E will do (blocks of one tile further apart than 2^19, values that would
+// move E over more than 2^60, or not finite; eight inputs of a query that are all below 2^-16 of its largest, whose parts would
+// lose bits, or not finite), the workgroup computes its rows with the f32 matrix instruction instead (attn_mx8_f32: one token
+// behind 4100 keys of the 8B shape 81 us for 11, 32 behind 480 35 for 15, 2048 1220 for 108).  So no row loses bits to a key that
+// it does not see.
 //
 // Probabilities are 2^(s - m) with a reference m of the row that lies MX_UP below its largest score, so that their f16 parts
 // stay normal.  m follows the largest score only when a tile passes it by MX_LAG: until then probabilities of up to

@@ -1172,6 +1172,7 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
     if (int e = need_room(a.q, qb, op, "q")) return e;
     if (int e = need_room(a.o, qb, op, "the output")) return e;
     const uint32_t cus = g_cus > 0 ? (uint32_t)g_cus : 1u;
+    // keys: the slots that may hold some.  How many do is the Paso's; the figures below are of caches that the keys fill.
     const uint64_t nrow = (uint64_t)T * G, keys = a.swa && (uint64_t)a.swa + T < a.rows ? a.swa + T : a.rows;
     // 8-bit caches: blocks of 128 rows, whose wavefronts share the unpacked tiles, where there are enough of them for the
     // device's CUs, five for two of them where every share of the keys has 512 (8B shape, 2048 tokens: 107 us, 151 with blocks
@@ -1196,7 +1197,8 @@ int attn_cache(const char* op, const Ctx& c, QpAttnArgs& a, uint32_t fmt, bool t
         // Shares of 256 keys or more (512 in blocks of 128 rows), while they make at most two workgroups for each CU; none
         // where the blocks alone are one for each (one token behind 4100 keys in 18 shares: 13.4 us, in 32 14.0).  Up to 8
         // shares may have 128 (32 tokens behind 480 keys: 11.3 us, 12.3 with two shares), unless all have 256 (25 tokens of a
-        // tree behind 96 keys: 7.8 us, 10.0 with two shares: their meeting costs 2 to 4).
+        // tree behind 96 keys: 7.8 us, 10.0 with two shares: their meeting costs 2 to 4).  In larger caches some shares are
+        // empty and are met all the same: those 32 tokens 14.8 us in 4096 slots, 30 in 131072; that tree 10.2 in 512.
         const uint32_t wgs = a.nkv * yb;
         const uint32_t share = wide ? 512 : 256, few = keys <= 256 ? 1 : std::min(8u, std::min(cus / wgs, cdiv(keys, 128)));
         ns = wgs >= cus ? 1 : std::max(few, std::min(cdiv(2 * cus, wgs), cdiv(keys, share)));
